@@ -16,3 +16,29 @@ def pytest_configure(config):
 @pytest.fixture(scope="session")
 def golden_dir():
     return os.path.join(REPO, "tests", "golden")
+
+
+# The plugin compiles against the reference's ggml headers and its tests run the reference's host
+# stack.  Where neither the built files nor the sources to build them are there, the tests that
+# need them are skipped, each by name, and the rest run.
+REF = "/root/reference"
+NEEDS_PLUGIN = {
+    "test_abi.py": {"test_plugin_exports_every_declared_symbol", "test_plugin_loads_and_scores_without_gpu",
+                    "test_plugin_is_gfx950_code_object"},
+    "test_bench_harness.py": {"test_replicas_two_ranks_with_split_series", "test_single_process_with_split_series"},
+    "test_gguf_synth.py": {"test_tiny_model_runs_on_reference_cpu"},
+    "test_refhost_drivers.py": None,   # all of it
+    "test_gpu_kernels.py": None,
+    "test_gpu_model.py": None,
+}
+
+
+def pytest_collection_modifyitems(config, items):
+    built = os.path.exists(os.path.join(REPO, "llamacog_amd", "libggml-mi355x.so"))
+    if built or os.path.exists(os.path.join(REF, "ggml", "include", "ggml.h")):
+        return
+    skip = pytest.mark.skip(reason=f"plugin not built and no ggml headers under {REF} to build it from")
+    for item in items:
+        names = NEEDS_PLUGIN.get(os.path.basename(str(item.fspath)), ())
+        if names is None or item.originalname in names:
+            item.add_marker(skip)
