@@ -21,6 +21,7 @@ extern "C" {
 
 typedef struct ggml_backend_reg * ggml_backend_reg_t;
 typedef struct ggml_backend *     ggml_backend_t;
+typedef struct ggml_backend_buffer_type * ggml_backend_buffer_type_t;
 
 // plugin entry points (GGML_BACKEND_DL)
 ggml_backend_reg_t ggml_backend_init(void);
@@ -129,6 +130,64 @@ double mi355x_bench_gemv(int wtype, int64_t K, int64_t M, int nmat, int copies, 
 // microbenchmark hook: which = 0 decode flash attention (D 128, H 32, Hkv 8, a cache
 // positions, b unmasked), 1 fused ADD+RMS_NORM+MUL+Q8_K of a floats; device us per launch
 double mi355x_bench_op(int which, int64_t a, int64_t b, int iters);
+
+// ---- operators on device tensors (llamacog_amd/csrc/devops_capi.cpp) -------------------------
+// MXFP4 products and expert routing.  They build no ggml node and need no ggml library: the plugin
+// exports them, and so does libmi355x-ops.so, which is these alone.  Pointers belong to the current
+// device.  stream: NULL as above, MI355X_STREAM_DEFAULT the device's default stream, otherwise a
+// stream, on which the work is queued and not waited for (a captured one too).  Returns 0 or a
+// code below, and then nothing was launched unless the code is MI355X_ERR_HIP.  Element types are
+// the ggml_type numbers 0 (f32), 1 (f16) and 30 (bf16); ld* are elements from one row to the next.
+#define MI355X_STREAM_DEFAULT ((void *) 1)
+#define MI355X_MX4 (-4)             // an operand given as MXFP4 codes and scales
+#define MI355X_ERR_TYPE (-1)
+#define MI355X_ERR_SHAPE (-2)
+#define MI355X_ERR_ALIGN (-3)       // codes, y and workspaces 16 bytes, scales 8, the rest its element
+#define MI355X_ERR_WORKSPACE (-4)
+#define MI355X_ERR_HIP (-5)
+
+// MXFP4 rows: codes [rows][K / 2], element 2 i in the low half of byte i, E2M1 (sign, then 0 0.5 1
+// 1.5 2 3 4 6); scales [ceil(K / 256)][rows][8], byte b of plane s the exponent of the row's elements
+// 256 s + 32 b to 256 s + 32 b + 31: 2^(byte - 127), 255 NaN.  K a multiple of 32; bytes past K have no
+// meaning (quantize sets them to 0).
+int64_t mi355x_mx4_scales_bytes(int64_t rows, int64_t K);
+// per block of 32: exponent floor(log2 max|x|) - 2, elements to nearest even, at most 6; a block
+// that holds an infinity or a NaN becomes NaN
+int mi355x_mx4_quantize(int xtype, const void * x, int64_t ldx, int64_t rows, int64_t K, uint8_t * codes, uint8_t * scales,
+                        void * stream);
+int mi355x_mx4_dequantize(const uint8_t * codes, const uint8_t * scales, int64_t rows, int64_t K, int ytype, void * y,
+                          void * stream);
+// y[T][M] = W[M][K] . x[T][K], W in MXFP4.  x as MXFP4 (xtype MI355X_MX4: x its codes, x_scales), or
+// as f32 / f16 / bf16 rows that the call quantises into the workspace first; sums in f32
+int64_t mi355x_mx4_mul_mat_workspace(int64_t T, int64_t K);
+int mi355x_mx4_mul_mat(const uint8_t * w_codes, const uint8_t * w_scales, int64_t M, int64_t K, int xtype, const void * x,
+                       const uint8_t * x_scales, int64_t ldx, int64_t T, int ytype, void * y, void * work, int64_t work_bytes,
+                       void * stream);
+// the experts' product on sorted pairs: y[p][M] = W[e][M][K] . x for offsets[e] <= p < offsets[e + 1],
+// with x row order[p] / used of x[T][K], or with x_sorted row p of x[T * used][K]; rows from
+// offsets[n_expert] on are set to zero.  The workspace is mi355x_mx4_mul_mat_workspace of x's rows
+int mi355x_mx4_mul_mat_id(const uint8_t * w_codes, const uint8_t * w_scales, int64_t M, int64_t K, int64_t n_expert, int xtype,
+                          const void * x, const uint8_t * x_scales, int64_t ldx, int64_t T, int64_t used, int x_sorted,
+                          const int32_t * order, const int32_t * offsets, int ytype, void * y, void * work,
+                          int64_t work_bytes, void * stream);
+// the pairs p = t * used + slot of ids[T][used] (int32 or int64: id_bytes 4 or 8) by expert, in their
+// own order within one: order[T * used] pairs, -1 from offsets[n_expert] on; rank[T][used] each pair's
+// place, -1 for an id outside 0 .. n_expert - 1; offsets[n_expert + 1].  n_expert up to 1024, used to 16
+int64_t mi355x_moe_sort_workspace(int64_t T, int64_t used, int64_t n_expert);
+int mi355x_moe_sort(const void * ids, int id_bytes, int64_t T, int64_t used, int64_t n_expert, int32_t * order, int32_t * rank,
+                    int32_t * offsets, void * work, int64_t work_bytes, void * stream);
+// xs[rank[t][j]] = x[t]; xs[T * used][D] is zero from offsets[n_expert] on
+int mi355x_moe_gather(int type, const void * x, int64_t ldx, int64_t T, int64_t D, int64_t used, const int32_t * order,
+                      const int32_t * rank, void * xs, void * stream);
+// y[t] = sum over j with rank[t][j] >= 0 of w[t][j] ys[rank[t][j]], in f32, slots in order; w NULL: of
+// ys[rank[t][j]], which is the gather's gradient
+int mi355x_moe_combine(int type, const void * ys, int64_t ldys, int64_t T, int64_t D, int64_t used, const int32_t * rank,
+                       const float * w, void * y, void * stream);
+// the combine's gradient: dys[rank[t][j]] = w[t][j] dy[t] (zero from offsets[n_expert] on), dw[t][j] =
+// dy[t] . ys[rank[t][j]] in f32 (zero where rank[t][j] < 0)
+int mi355x_moe_combine_back(int type, const void * dy, int64_t lddy, const void * ys, int64_t ldys, int64_t T, int64_t D,
+                            int64_t used, const int32_t * order, const int32_t * rank, const float * w, void * dys, float * dw,
+                            void * stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,79 @@
+// devops.h — the operators on device tensors that stand outside the ggml graph: MXFP4 products
+// and expert routing (k_mx4.hip, k_moe.hip, devops_capi.cpp).
+//
+// These sources need no ggml header: they are linked into the plugin beside the rest and, alone,
+// into libmi355x-ops.so for hosts that only call the flat ABI.  Nothing here aborts: a launcher
+// returns the HIP status of its launch and the C entry hands it on.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+#include <type_traits>
+
+namespace mi355x_ops {
+
+// element types of the flat ABI (the ggml_type numbers)
+enum elem_type { ELEM_F32 = 0, ELEM_F16 = 1, ELEM_BF16 = 30 };
+
+constexpr int MX4_BLOCK = 32;    // elements that share one exponent
+constexpr int MX4_PLANE = 256;   // elements whose eight exponents lie side by side
+constexpr int MOE_MAX_EXPERTS = 1024;
+constexpr int MOE_MAX_USED = 16;
+
+// MXFP4 rows: codes [rows][K / 2], element 2 i in the low half of byte i; scales
+// [ceil(K / 256)][rows][8].  Bytes of a scale plane that lie past K are never used.
+struct mx4_mat {
+    const uint8_t * codes;
+    const uint8_t * scales;
+    int64_t rows;
+    int64_t K;
+};
+
+// the sorted pairs of a routing step: pairs [offsets[e], offsets[e + 1]) belong to expert e
+struct moe_view {
+    const int32_t * order;     // [pairs] pair (token * used + slot) at a sorted place, -1 behind offsets[n_expert]
+    const int32_t * offsets;   // [n_expert + 1]
+    int64_t pairs;
+    int n_expert;
+    int used;                  // slots per token; 0: the product's rows are in sorted order already
+};
+
+hipError_t mx4_quantize(int type, const void * x, int64_t ldx, int64_t rows, int64_t K, uint8_t * codes, uint8_t * scales,
+                        hipStream_t st);
+hipError_t mx4_dequantize(const mx4_mat & m, int type, void * y, hipStream_t st);
+// y [T][M] = W . x for MXFP4 rows x
+hipError_t mx4_product(const mx4_mat & w, const mx4_mat & x, int ytype, void * y, hipStream_t st);
+// y [pairs][M]: sorted row p is expert e(p)'s W times x row order[p] / used (or p)
+hipError_t mx4_product_id(const mx4_mat & w, const mx4_mat & x, const moe_view & v, int ytype, void * y, hipStream_t st);
+
+size_t moe_sort_workspace(int64_t pairs, int n_expert);
+hipError_t moe_sort(const void * ids, int id_bytes, int64_t pairs, int n_expert, int32_t * order, int32_t * rank,
+                    int32_t * offsets, void * work, hipStream_t st);
+hipError_t moe_gather(int type, const void * x, int64_t ldx, int64_t T, int64_t D, int used, const int32_t * order,
+                      const int32_t * rank, void * xs, hipStream_t st);
+hipError_t moe_combine(int type, const void * ys, int64_t ldys, int64_t T, int64_t D, int used, const int32_t * rank,
+                       const float * w, void * y, hipStream_t st);
+hipError_t moe_combine_back(int type, const void * dy, int64_t lddy, const void * ys, int64_t ldys, int64_t T, int64_t D,
+                            int used, const int32_t * order, const int32_t * rank, const float * w, void * dys, float * dw,
+                            hipStream_t st);
+
+// ---- device side -----------------------------------------------------------------------------
+template <class T> __device__ __forceinline__ float to_f32(T v) { return (float) v; }
+template <class T> __device__ __forceinline__ T from_f32(float v) { return (T) v; }   // to nearest, ties to even
+
+// N elements moved as one access (N * sizeof(T) <= 16 and a power of two) and widened to float
+template <class T, int N> struct alignas(sizeof(T) * N) pack { T v[N]; };
+
+// a type as a template argument out of a run-time number: f(T{}) with T = float, _Float16 or __bf16
+template <class F> static inline hipError_t with_type(int type, F && f) {
+    switch (type) {
+        case ELEM_F32: return f(float{});
+        case ELEM_F16: return f(_Float16{});
+        case ELEM_BF16: return f(__bf16{});
+        default: return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace mi355x_ops

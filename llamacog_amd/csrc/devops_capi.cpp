@@ -1,0 +1,223 @@
+// devops_capi.cpp — the flat C ABI of the operators in devops.h: argument checks, streams and
+// workspaces.  Every entry returns 0 or a negative code (include/ggml-mi355x.h) and launches
+// nothing when it refuses; none aborts or throws.
+#include "devops.h"
+
+#include "../../include/ggml-mi355x.h"
+
+using namespace mi355x_ops;
+
+#define OPS_API extern "C" __attribute__((visibility("default")))
+
+namespace {
+
+// NULL: a private stream, waited for before the call returns; MI355X_STREAM_DEFAULT: the device's
+// default stream; anything else as it is, not waited for
+struct call_stream {
+    hipStream_t st = nullptr;
+    bool own = false;
+    hipError_t err = hipSuccess;
+    explicit call_stream(void * s) {
+        if (s == MI355X_STREAM_DEFAULT) return;
+        if (s) {
+            st = (hipStream_t) s;
+        } else {
+            err = hipStreamCreateWithFlags(&st, hipStreamNonBlocking);
+            own = err == hipSuccess;
+        }
+    }
+    ~call_stream() {
+        if (own) (void) hipStreamDestroy(st);
+    }
+    int done(hipError_t e) {
+        if (e == hipSuccess && own) e = hipStreamSynchronize(st);
+        return e == hipSuccess ? 0 : MI355X_ERR_HIP;
+    }
+};
+
+bool is_elem(int t) { return t == ELEM_F32 || t == ELEM_F16 || t == ELEM_BF16; }
+int64_t elem_size(int t) { return t == ELEM_F32 ? 4 : 2; }
+bool aligned(const void * p, uintptr_t n) { return (uintptr_t) p % n == 0; }
+
+constexpr int64_t MAX_K = (int64_t) 1 << 24;       // elements of a row
+constexpr int64_t MAX_ROWS = (int64_t) 1 << 31;    // rows of a matrix, pairs of a routing step (exclusive)
+
+int check_rows(int64_t rows, int64_t K) {
+    if (rows < 0 || rows >= MAX_ROWS) return MI355X_ERR_SHAPE;
+    if (K <= 0 || K % MX4_BLOCK || K > MAX_K) return MI355X_ERR_SHAPE;
+    return 0;
+}
+
+// codes are read 16 bytes at a time, exponents 8
+int check_mx4(const void * codes, const void * scales) {
+    return aligned(codes, 16) && aligned(scales, 8) ? 0 : MI355X_ERR_ALIGN;
+}
+
+int check_elems(int type, const void * p) {
+    if (!is_elem(type)) return MI355X_ERR_TYPE;
+    return aligned(p, (uintptr_t) elem_size(type)) ? 0 : MI355X_ERR_ALIGN;
+}
+
+// y rows are stored up to 16 bytes at a time where M allows it, which asks for a base to match
+int check_out(int type, const void * p) {
+    if (!is_elem(type)) return MI355X_ERR_TYPE;
+    return aligned(p, 16) ? 0 : MI355X_ERR_ALIGN;
+}
+
+int check_routing(int64_t T, int64_t used) {
+    if (T < 0 || used <= 0 || used > MOE_MAX_USED || T * used >= MAX_ROWS) return MI355X_ERR_SHAPE;
+    return 0;
+}
+
+int64_t codes_bytes(int64_t rows, int64_t K) { return (rows * (K / 2) + 255) / 256 * 256; }
+int64_t scales_bytes(int64_t rows, int64_t K) { return (K + MX4_PLANE - 1) / MX4_PLANE * rows * 8; }
+
+#define TRY(expr)                    \
+    do {                             \
+        const int rc_ = (expr);      \
+        if (rc_) return rc_;         \
+    } while (0)
+
+}  // namespace
+
+OPS_API int64_t mi355x_mx4_scales_bytes(int64_t rows, int64_t K) { return check_rows(rows, K) ? -1 : scales_bytes(rows, K); }
+
+OPS_API int mi355x_mx4_quantize(int xtype, const void * x, int64_t ldx, int64_t rows, int64_t K, uint8_t * codes,
+                                uint8_t * scales, void * stream) {
+    TRY(check_rows(rows, K));
+    TRY(check_elems(xtype, x));
+    TRY(check_mx4(codes, scales));
+    if (ldx < K && rows > 1) return MI355X_ERR_SHAPE;
+    if (rows == 0) return 0;
+    call_stream cs(stream);
+    if (cs.err != hipSuccess) return MI355X_ERR_HIP;
+    return cs.done(mx4_quantize(xtype, x, ldx, rows, K, codes, scales, cs.st));
+}
+
+OPS_API int mi355x_mx4_dequantize(const uint8_t * codes, const uint8_t * scales, int64_t rows, int64_t K, int ytype, void * y,
+                                  void * stream) {
+    TRY(check_rows(rows, K));
+    TRY(check_out(ytype, y));
+    TRY(check_mx4(codes, scales));
+    if (rows == 0) return 0;
+    call_stream cs(stream);
+    if (cs.err != hipSuccess) return MI355X_ERR_HIP;
+    return cs.done(mx4_dequantize({codes, scales, rows, K}, ytype, y, cs.st));
+}
+
+OPS_API int64_t mi355x_mx4_mul_mat_workspace(int64_t T, int64_t K) {
+    return check_rows(T, K) ? -1 : codes_bytes(T, K) + scales_bytes(T, K);
+}
+
+// the x operand of a product: MXFP4 as given, or quantised into the workspace
+static int x_operand(int xtype, const void * x, const uint8_t * xscales, int64_t ldx, int64_t rows, int64_t K, void * work,
+                     int64_t work_bytes, hipStream_t st, mx4_mat & m) {
+    if (xtype == MI355X_MX4) {
+        m = {(const uint8_t *) x, xscales, rows, K};
+        return 0;
+    }
+    uint8_t * codes = (uint8_t *) work, * scales = codes + codes_bytes(rows, K);
+    m = {codes, scales, rows, K};
+    return mx4_quantize(xtype, x, ldx, rows, K, codes, scales, st) == hipSuccess ? 0 : MI355X_ERR_HIP;
+}
+
+static int check_x(int xtype, const void * x, const uint8_t * xscales, int64_t ldx, int64_t rows, int64_t K, const void * work,
+                   int64_t work_bytes) {
+    TRY(check_rows(rows, K));
+    if (xtype == MI355X_MX4) return check_mx4(x, xscales);
+    TRY(check_elems(xtype, x));
+    if (ldx < K && rows > 1) return MI355X_ERR_SHAPE;
+    if (!aligned(work, 16)) return MI355X_ERR_ALIGN;
+    return work_bytes >= codes_bytes(rows, K) + scales_bytes(rows, K) ? 0 : MI355X_ERR_WORKSPACE;
+}
+
+OPS_API int mi355x_mx4_mul_mat(const uint8_t * w_codes, const uint8_t * w_scales, int64_t M, int64_t K, int xtype,
+                               const void * x, const uint8_t * x_scales, int64_t ldx, int64_t T, int ytype, void * y,
+                               void * work, int64_t work_bytes, void * stream) {
+    TRY(check_rows(M, K));
+    TRY(check_mx4(w_codes, w_scales));
+    TRY(check_x(xtype, x, x_scales, ldx, T, K, work, work_bytes));
+    TRY(check_out(ytype, y));
+    if (T == 0 || M == 0) return 0;
+    call_stream cs(stream);
+    if (cs.err != hipSuccess) return MI355X_ERR_HIP;
+    mx4_mat xm;
+    TRY(x_operand(xtype, x, x_scales, ldx, T, K, work, work_bytes, cs.st, xm));
+    return cs.done(mx4_product({w_codes, w_scales, M, K}, xm, ytype, y, cs.st));
+}
+
+OPS_API int mi355x_mx4_mul_mat_id(const uint8_t * w_codes, const uint8_t * w_scales, int64_t M, int64_t K, int64_t n_expert,
+                                  int xtype, const void * x, const uint8_t * x_scales, int64_t ldx, int64_t T, int64_t used,
+                                  int x_sorted, const int32_t * order, const int32_t * offsets, int ytype, void * y,
+                                  void * work, int64_t work_bytes, void * stream) {
+    TRY(check_rows(M, K));
+    TRY(check_mx4(w_codes, w_scales));
+    TRY(check_routing(T, used));
+    if (n_expert <= 0 || n_expert > MOE_MAX_EXPERTS) return MI355X_ERR_SHAPE;
+    const int64_t rows = x_sorted ? T * used : T;
+    TRY(check_x(xtype, x, x_scales, ldx, rows, K, work, work_bytes));
+    TRY(check_out(ytype, y));
+    if (T == 0 || M == 0) return 0;
+    call_stream cs(stream);
+    if (cs.err != hipSuccess) return MI355X_ERR_HIP;
+    mx4_mat xm;
+    TRY(x_operand(xtype, x, x_scales, ldx, rows, K, work, work_bytes, cs.st, xm));
+    const moe_view v = {order, offsets, T * used, (int) n_expert, x_sorted ? 0 : (int) used};
+    return cs.done(mx4_product_id({w_codes, w_scales, M, K}, xm, v, ytype, y, cs.st));
+}
+
+OPS_API int64_t mi355x_moe_sort_workspace(int64_t T, int64_t used, int64_t n_expert) {
+    if (check_routing(T, used) || n_expert <= 0 || n_expert > MOE_MAX_EXPERTS) return -1;
+    return (int64_t) moe_sort_workspace(T * used, (int) n_expert);
+}
+
+OPS_API int mi355x_moe_sort(const void * ids, int id_bytes, int64_t T, int64_t used, int64_t n_expert, int32_t * order,
+                            int32_t * rank, int32_t * offsets, void * work, int64_t work_bytes, void * stream) {
+    TRY(check_routing(T, used));
+    if (n_expert <= 0 || n_expert > MOE_MAX_EXPERTS) return MI355X_ERR_SHAPE;
+    if (id_bytes != 4 && id_bytes != 8) return MI355X_ERR_TYPE;
+    if (!aligned(ids, id_bytes) || !aligned(work, 4)) return MI355X_ERR_ALIGN;
+    if (work_bytes < (int64_t) moe_sort_workspace(T * used, (int) n_expert)) return MI355X_ERR_WORKSPACE;
+    call_stream cs(stream);
+    if (cs.err != hipSuccess) return MI355X_ERR_HIP;
+    return cs.done(moe_sort(ids, id_bytes, T * used, (int) n_expert, order, rank, offsets, work, cs.st));
+}
+
+OPS_API int mi355x_moe_gather(int type, const void * x, int64_t ldx, int64_t T, int64_t D, int64_t used, const int32_t * order,
+                              const int32_t * rank, void * xs, void * stream) {
+    TRY(check_routing(T, used));
+    TRY(check_elems(type, x));
+    TRY(check_elems(type, xs));
+    if (D < 0 || D > MAX_K || (ldx < D && T > 1)) return MI355X_ERR_SHAPE;
+    if (T == 0 || D == 0) return 0;
+    call_stream cs(stream);
+    if (cs.err != hipSuccess) return MI355X_ERR_HIP;
+    return cs.done(moe_gather(type, x, ldx, T, D, (int) used, order, rank, xs, cs.st));
+}
+
+OPS_API int mi355x_moe_combine(int type, const void * ys, int64_t ldys, int64_t T, int64_t D, int64_t used,
+                               const int32_t * rank, const float * w, void * y, void * stream) {
+    TRY(check_routing(T, used));
+    TRY(check_elems(type, ys));
+    TRY(check_elems(type, y));
+    if (D < 0 || D > MAX_K || (ldys < D && T * used > 1)) return MI355X_ERR_SHAPE;
+    if (T == 0 || D == 0) return 0;
+    call_stream cs(stream);
+    if (cs.err != hipSuccess) return MI355X_ERR_HIP;
+    return cs.done(moe_combine(type, ys, ldys, T, D, (int) used, rank, w, y, cs.st));
+}
+
+OPS_API int mi355x_moe_combine_back(int type, const void * dy, int64_t lddy, const void * ys, int64_t ldys, int64_t T,
+                                    int64_t D, int64_t used, const int32_t * order, const int32_t * rank, const float * w,
+                                    void * dys, float * dw, void * stream) {
+    TRY(check_routing(T, used));
+    TRY(check_elems(type, dy));
+    TRY(check_elems(type, ys));
+    TRY(check_elems(type, dys));
+    if (D < 0 || D > MAX_K || (lddy < D && T > 1) || (ldys < D && T * used > 1)) return MI355X_ERR_SHAPE;
+    if (!w) return MI355X_ERR_SHAPE;
+    if (T == 0) return 0;
+    call_stream cs(stream);
+    if (cs.err != hipSuccess) return MI355X_ERR_HIP;
+    return cs.done(moe_combine_back(type, dy, lddy, ys, ldys, T, D, (int) used, order, rank, w, dys, dw, cs.st));
+}

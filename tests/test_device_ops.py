@@ -1,0 +1,619 @@
+"""The operators on device tensors (llamacog_amd.device_ops): MXFP4 quantisation and products, expert
+sort, gather, combine and their gradients, against plain numpy in 64 bits.
+
+Tolerances are bounds, not fits.  Quantisation, values, sorting and gathering are exact.  A product
+adds K products of at most 4 significant bits each (exact in float32) in some order: each of fewer
+than K additions rounds by at most 2^-24 of a partial sum that sum |w x| bounds, hence
+K 2^-24 sum |w x|, and the result is rounded once to y's type (half a step: eps / 2).  A combine adds
+`used` rounded products: (2 used) 2^-24 sum |w y|, and so on."""
+import ctypes
+import os
+import re
+import subprocess
+
+import numpy as np
+import pytest
+import torch
+
+import llamacog_amd as la
+from llamacog_amd import device_ops as ops
+
+gpu = pytest.mark.gpu
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+GRID = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6, -0.0, -0.5, -1, -1.5, -2, -3, -4, -6])
+U32 = 2.0 ** -24
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+def least_step(t):
+    """Half a step below the normal range, where steps stop shrinking: a rounding to t there is off by
+    at most this, however small the number (float16: 2^-25)."""
+    return torch.finfo(t).smallest_normal * torch.finfo(t).eps / 2
+
+
+# ---- plain forms ---------------------------------------------------------------------------------
+def np_quantize(x):
+    """float64 [rows, K] -> (codes [rows, K], exponent bytes [rows, K / 32])."""
+    b = x.reshape(x.shape[0], -1, 32)
+    top = np.abs(b).max(-1)
+    finite = np.isfinite(b).all(-1)
+    safe = np.where(finite & (top > 0), top, 1.0)
+    e = np.clip(np.where(top > 0, np.frexp(safe)[1] - 3, -127), -127, 127)
+    with np.errstate(invalid="ignore"):
+        a = np.abs(b) * np.exp2(-e.astype(np.float64))[..., None]
+        r = np.where(a < 2, np.rint(a * 2) / 2, np.where(a < 4, np.rint(a), np.rint(a / 2) * 2))
+    r = np.where(finite[..., None], np.minimum(r, 6), 0)
+    code = np.where(r < 2, r * 2, np.where(r < 4, r + 2, r / 2 + 4)).astype(np.uint8)
+    code |= ((np.signbit(b) & finite[..., None]).astype(np.uint8) << 3)
+    return code.reshape(x.shape), np.where(finite, e + 127, 255).astype(np.uint8)
+
+
+def np_values(code, e):
+    s = np.where(e == 255, np.nan, np.exp2(e.astype(np.float64) - 127))
+    return (GRID[code].reshape(*e.shape, 32) * s[..., None]).reshape(code.shape)
+
+
+def np_rounded(x):
+    return np_values(*np_quantize(x))
+
+
+def pack(code, e):
+    """codes and exponent bytes [..., rows, *] -> Mx4 on the GPU; the bytes past K hold rubbish."""
+    rows, nb = e.shape[-2:]
+    planes = np.full(e.shape[:-1] + (-(-nb // 8) * 8,), 0xFF, np.uint8)
+    planes[..., :nb] = e
+    planes = np.moveaxis(planes.reshape(e.shape[:-1] + (-1, 8)), -2, -3)
+    both = code[..., 0::2] | (code[..., 1::2] << 4)
+    return ops.Mx4(torch.from_numpy(np.ascontiguousarray(both)).cuda(), torch.from_numpy(np.ascontiguousarray(planes)).cuda())
+
+
+def unpack(m):
+    c, s = m.codes.cpu().numpy(), m.scales.cpu().numpy()
+    code = np.stack((c & 15, c >> 4), -1).reshape(*c.shape[:-1], -1)
+    e = np.moveaxis(s, -3, -2).reshape(*s.shape[:-3], s.shape[-2], -1)[..., : code.shape[-1] // 32]
+    return code, e
+
+
+def random_mx4(rng, *shape):
+    """Random codes and exponents of a few octaves: (Mx4, values in 64 bits)."""
+    code = rng.integers(0, 16, shape, dtype=np.uint8)
+    e = rng.integers(120, 130, shape[:-1] + (shape[-1] // 32,), dtype=np.uint8)
+    return pack(code, e), np_values(code, e)
+
+
+def rows_of(rng, rows, k, dtype):
+    x = torch.from_numpy(rng.standard_normal((rows, k)) * (1 + 8 * (rng.random(k) < 0.02))).to(dtype).cuda()
+    return x, x.double().cpu().numpy()
+
+
+def check_product(y, w, x, dtype, what=""):
+    """y against x w^T in 64 bits within the bound of the docstring."""
+    got, want = y.double().cpu().numpy(), x @ w.T
+    room = np.abs(x) @ np.abs(w).T * w.shape[1] * U32
+    off = np.abs(got - want) - room - half_step(dtype) * (np.abs(want) + room) - least_step(dtype)
+    assert not np.isnan(got).any() and off.max(initial=-1) <= 0, f"{what}: off by {off.max():.3g} more than the bound"
+
+
+def np_sort(ids, n_expert):
+    flat = ids.reshape(-1)
+    held = [(e, p) for p, e in enumerate(flat) if 0 <= e < n_expert]
+    order = [p for _, p in sorted(held)]
+    rank = np.full(flat.shape, -1, np.int32)
+    rank[order] = np.arange(len(order))
+    offsets = np.searchsorted(np.sort(np.array([e for e, _ in held], int)), np.arange(n_expert + 1))
+    return np.array(order + [-1] * (flat.size - len(order)), np.int32), rank.reshape(ids.shape), offsets.astype(np.int32)
+
+
+def routing(rng, t, used, n_expert, kind):
+    if kind == "one":        # everything to one expert
+        return np.full((t, used), n_expert - 1)
+    if kind == "none":       # padding only
+        return np.full((t, used), -1)
+    ids = rng.integers(0, n_expert, (t, used))   # the same expert twice for a token now and then
+    if kind == "holes":
+        ids[rng.random((t, used)) < 0.3] = -1
+        ids[rng.random((t, used)) < 0.1] = n_expert
+        ids[-max(1, t // 4):] = -7
+    return ids
+
+
+# ---- without a GPU -------------------------------------------------------------------------------
+def test_library_exports_what_the_header_declares():
+    text = re.sub(r"//.*", "", open(os.path.join(la.REPO, "include", "ggml-mi355x.h")).read())
+    names = set(re.findall(r"\bmi355x_(?:mx4|moe)_\w+(?=\s*\()", text))
+    assert names == {n for n in ops._SIGNATURES}
+    out = subprocess.run(["nm", "-D", "--defined-only", ops.LIBRARY], capture_output=True, text=True, check=True).stdout
+    exported = {line.split()[-1] for line in out.splitlines() if " T " in line}
+    assert exported == names   # nothing else, so that the plugin's copy of the kernels stays apart
+    assert b"gfx950" in open(ops.LIBRARY, "rb").read()
+
+
+@pytest.mark.parametrize("compiler,language", [("gcc", "c"), ("g++", "c++")])
+def test_header_stands_alone(tmp_path, compiler, language):
+    src = tmp_path / "t"
+    src.write_text('#include "ggml-mi355x.h"\nint main(void) { return mi355x_moe_sort_workspace(1, 1, 1) != 0; }\n')
+    subprocess.run([compiler, "-x", language, "-Wall", "-Werror", "-fsyntax-only", "-I", os.path.join(la.REPO, "include"), str(src)],
+                   check=True)
+
+
+A = 1 << 20   # an aligned address that no call below gets to read
+
+REFUSED = [
+    ("mi355x_mx4_quantize", (2, A, 64, 3, 64, A, A), -1),                # type
+    ("mi355x_mx4_quantize", (0, A, 64, 3, 48, A, A), -2),                # K not of whole blocks
+    ("mi355x_mx4_quantize", (0, A, 64, 3, 0, A, A), -2),
+    ("mi355x_mx4_quantize", (0, A, 64, -1, 64, A, A), -2),
+    ("mi355x_mx4_quantize", (0, A, 32, 3, 64, A, A), -2),                # rows that overlap
+    ("mi355x_mx4_quantize", (0, A, 64, 3, 1 << 25, A, A), -2),
+    ("mi355x_mx4_quantize", (0, A, 64, 1 << 31, 64, A, A), -2),
+    ("mi355x_mx4_quantize", (0, A + 2, 64, 3, 64, A, A), -3),
+    ("mi355x_mx4_quantize", (1, A, 64, 3, 64, A + 8, A), -3),
+    ("mi355x_mx4_quantize", (1, A, 64, 3, 64, A, A + 4), -3),
+    ("mi355x_mx4_dequantize", (A, A, 3, 64, 39, A), -1),
+    ("mi355x_mx4_dequantize", (A, A, 3, 40, 0, A), -2),
+    ("mi355x_mx4_dequantize", (A, A, 3, 64, 0, A + 4), -3),
+    ("mi355x_mx4_mul_mat", (A, A, 8, 64, 12, A, None, 64, 3, 0, A, A, 1 << 20), -1),
+    ("mi355x_mx4_mul_mat", (A, A, 8, 64, 0, A, None, 64, 3, 8, A, A, 1 << 20), -1),
+    ("mi355x_mx4_mul_mat", (A, A, 8, 65, 0, A, None, 64, 3, 0, A, A, 1 << 20), -2),
+    ("mi355x_mx4_mul_mat", (A, A, 8, 64, 0, A, None, 63, 3, 0, A, A, 1 << 20), -2),
+    ("mi355x_mx4_mul_mat", (A + 1, A, 8, 64, 0, A, None, 64, 3, 0, A, A, 1 << 20), -3),
+    ("mi355x_mx4_mul_mat", (A, A, 8, 64, -4, A, A + 2, 64, 3, 0, A, None, 0), -3),
+    ("mi355x_mx4_mul_mat", (A, A, 8, 64, 0, A, None, 64, 3, 0, A, A, 100), -4),
+    ("mi355x_mx4_mul_mat_id", (A, A, 8, 64, 0, 0, A, None, 64, 3, 2, 0, A, A, 0, A, A, 1 << 20), -2),
+    ("mi355x_mx4_mul_mat_id", (A, A, 8, 64, 1025, 0, A, None, 64, 3, 2, 0, A, A, 0, A, A, 1 << 20), -2),
+    ("mi355x_mx4_mul_mat_id", (A, A, 8, 64, 4, 0, A, None, 64, 3, 17, 0, A, A, 0, A, A, 1 << 20), -2),
+    ("mi355x_mx4_mul_mat_id", (A, A, 8, 64, 4, 0, A, None, 64, 3, 2, 1, A, A, 0, A, A, 303), -4),
+    ("mi355x_moe_sort", (A, 4, 3, 0, 4, A, A, A, None, 0), -2),
+    ("mi355x_moe_sort", (A, 4, 1 << 30, 2, 4, A, A, A, None, 0), -2),
+    ("mi355x_moe_sort", (A, 2, 3, 2, 4, A, A, A, None, 0), -1),
+    ("mi355x_moe_sort", (A + 4, 8, 3, 2, 4, A, A, A, None, 0), -3),
+    ("mi355x_moe_sort", (A, 4, 1 << 20, 2, 4, A, A, A, None, 0), -4),
+    ("mi355x_moe_gather", (0, A, 8, 3, 9, 2, A, A, A), -2),
+    ("mi355x_moe_gather", (0, A + 1, 9, 3, 9, 2, A, A, A), -3),
+    ("mi355x_moe_combine", (5, A, 9, 3, 9, 2, A, A, A), -1),
+    ("mi355x_moe_combine", (0, A, 9, 3, -1, 2, A, A, A), -2),
+    ("mi355x_moe_combine_back", (0, A, 8, A, 9, 3, 9, 2, A, A, A, A, A), -2),
+    ("mi355x_moe_combine_back", (0, A, 9, A, 9, 3, 9, 2, A, A, None, A, A), -2),
+    ("mi355x_moe_combine_back", (1, A, 9, A, 9, 3, 9, 2, A, A, A, A + 1, A), -3),
+]
+
+
+@pytest.mark.parametrize("name,args,code", REFUSED, ids=[f"{n[7:]}-{i}" for i, (n, _, _) in enumerate(REFUSED)])
+def test_flat_calls_refused_before_any_launch(name, args, code):
+    assert getattr(ops.library(), name)(*args, None) == code
+
+
+EMPTY = [
+    ("mi355x_mx4_quantize", (0, A, 64, 0, 64, A, A)),
+    ("mi355x_mx4_dequantize", (A, A, 0, 64, 0, A)),
+    ("mi355x_mx4_mul_mat", (A, A, 8, 64, 0, A, None, 64, 0, 0, A, A, 0)),
+    ("mi355x_mx4_mul_mat", (A, A, 0, 64, 0, A, None, 64, 3, 0, A, A, 1 << 20)),
+    ("mi355x_mx4_mul_mat_id", (A, A, 8, 64, 4, 0, A, None, 64, 0, 2, 0, A, A, 0, A, A, 0)),
+    ("mi355x_moe_gather", (0, A, 9, 0, 9, 2, A, A, A)),
+    ("mi355x_moe_combine", (0, A, 9, 3, 0, 2, A, A, A)),
+    ("mi355x_moe_combine_back", (0, A, 9, A, 9, 0, 9, 2, A, A, A, A, A)),
+]
+
+
+@pytest.mark.parametrize("name,args", EMPTY, ids=[f"{n[7:]}-{i}" for i, (n, _) in enumerate(EMPTY)])
+def test_flat_calls_with_nothing_to_do(name, args):
+    assert getattr(ops.library(), name)(*args, None) == 0
+
+
+def test_sizes():
+    lib = ops.library()
+    assert lib.mi355x_mx4_scales_bytes(3, 288) == 2 * 3 * 8 and lib.mi355x_mx4_scales_bytes(3, 289) == -1
+    assert lib.mi355x_mx4_mul_mat_workspace(3, 288) == 512 + 48
+    assert lib.mi355x_moe_sort_workspace(10, 2, 8) == 0 and lib.mi355x_moe_sort_workspace(1, 17, 8) == -1
+    assert lib.mi355x_moe_sort_workspace(1 << 20, 2, 8) > 0
+
+
+def test_tensors_of_the_host_are_refused():
+    x, ids = torch.zeros(2, 64), torch.zeros(2, 2, dtype=torch.int32)
+    m = ops.Mx4(torch.zeros(2, 32, dtype=torch.uint8), torch.zeros(1, 2, 8, dtype=torch.uint8))
+    plan = ops.MoePlan(torch.zeros(4, dtype=torch.int32), ids, torch.zeros(5, dtype=torch.int32))
+    for call in (lambda: ops.mx4_quantize(x), lambda: ops.mx4_dequantize(m), lambda: ops.mx4_mul_mat(m, x),
+                 lambda: ops.mx4_mul_mat_id(m, x, plan), lambda: ops.moe_sort(ids, 4), lambda: ops.moe_gather(x, plan),
+                 lambda: ops.moe_combine(x, plan), lambda: ops.moe_combine_back(x, x, plan, x)):
+        with pytest.raises(ValueError, match="on an MI355X is wanted"):
+            call()
+    with pytest.raises(TypeError):
+        ops.mx4_mul_mat(x, x)
+    with pytest.raises(TypeError):
+        ops.mx4_quantize(np.zeros((2, 64), np.float32))
+
+
+# ---- MXFP4 ---------------------------------------------------------------------------------------
+def special_blocks():
+    """Blocks at the edges: zeros, ties, the largest and least numbers, infinities and NaNs."""
+    rng = np.random.default_rng(5)
+    b = [np.zeros(32), -np.zeros(32), np.full(32, 2.0 ** -149), np.linspace(-6, 6, 32), np.full(32, 7.99), np.full(32, 3.4e38)]
+    b.append(np.concatenate(([4.0], (np.arange(31) - 15) * 0.25)))     # ties of every step, kept by the 4
+    b.append(np.concatenate(([6.5], (np.arange(31) - 15) * 0.5)))
+    b += [rng.standard_normal(32) * 2.0 ** e for e in (-140, -127, -126, -125, -124, -20, 100, 124)]
+    for bad in (np.inf, -np.inf, np.nan):
+        v = rng.standard_normal(32)
+        v[rng.integers(32)] = bad
+        b.append(v)
+    return np.array(b, np.float32).reshape(1, -1)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_quantize_special_blocks(dtype):
+    x = torch.from_numpy(special_blocks()).to(dtype)
+    code, e = unpack(ops.mx4_quantize(x.cuda()))
+    want_code, want_e = np_quantize(x.double().numpy())
+    assert (e == want_e).all() and (code == want_code).all()
+    for out in TYPES:
+        y = ops.mx4_dequantize(ops.mx4_quantize(x.cuda()), out).cpu()
+        assert torch.equal(y.nan_to_num(99.0), torch.from_numpy(np_values(code, e)).to(out).nan_to_num(99.0))
+        assert torch.equal(y.isnan(), torch.from_numpy(np_values(code, e)).isnan())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,k", [(1, 32), (3, 64), (17, 96), (5, 288), (1, 4096), (33, 1056), (257, 2048), (2, 14336)])
+def test_quantize(rows, k, dtype):
+    rng = np.random.default_rng(rows * k)
+    x, x64 = rows_of(rng, rows, k, dtype)
+    m = ops.mx4_quantize(x)
+    code, e = unpack(m)
+    want_code, want_e = np_quantize(x64)
+    assert (e == want_e).all() and (code == want_code).all()
+    if k % 256:
+        assert int(m.scales[-1, :, k // 32 % 8:].sum()) == 0
+    assert torch.equal(ops.mx4_dequantize(m).double().cpu(), torch.from_numpy(np_values(code, e)))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("first", [0, 1, 4, 8])
+def test_quantize_strided_rows(dtype, first):
+    rng = np.random.default_rng(7)
+    big, _ = rows_of(rng, 9, 333, dtype)
+    x = big[1::2, first:first + 288]
+    assert not x.is_contiguous()
+    a, b = ops.mx4_quantize(x), ops.mx4_quantize(x.contiguous())
+    assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+
+
+PRODUCTS = [(1, 16, 32), (1, 17, 4096), (1, 4096, 544), (2, 5, 64), (3, 33, 288), (15, 64, 256), (16, 16, 512), (17, 100, 2080),
+            (31, 257, 1024), (33, 48, 96), (64, 130, 768), (65, 1, 320), (129, 300, 1280), (300, 129, 224), (512, 1000, 576)]
+
+
+@gpu
+@pytest.mark.parametrize("t,m,k", PRODUCTS)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_product(t, m, k, dtype):
+    rng = np.random.default_rng(t * m + k)
+    w, w64 = random_mx4(rng, m, k)
+    x, x64 = rows_of(rng, t, k, dtype)
+    y = ops.mx4_mul_mat(w, x)
+    assert y.dtype == dtype and y.shape == (t, m)
+    check_product(y, w64, np_rounded(x64), dtype)
+    # quantised by the caller, and to another type
+    assert torch.equal(ops.mx4_mul_mat(w, ops.mx4_quantize(x), dtype), y)
+    check_product(ops.mx4_mul_mat(w, x, torch.float32), w64, np_rounded(x64), torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("t", [1, 5, 100, 400])
+def test_product_strided_rows(t):
+    rng = np.random.default_rng(t)
+    w, _ = random_mx4(rng, 70, 288)
+    big, _ = rows_of(rng, 2 * t, 300, torch.float16)
+    x = big[::2, 3:291]
+    assert torch.equal(ops.mx4_mul_mat(w, x), ops.mx4_mul_mat(w, x.contiguous()))
+
+
+@gpu
+@pytest.mark.parametrize("t,m,k", [(1, 40, 512), (20, 40, 544), (300, 300, 544)])
+def test_product_nan_blocks_stay_in_their_row(t, m, k):
+    rng = np.random.default_rng(3)
+    code, e = rng.integers(0, 16, (m, k), dtype=np.uint8), rng.integers(120, 130, (m, k // 32), dtype=np.uint8)
+    e[m // 2, -1] = 255
+    x, x64 = rows_of(rng, t, k, torch.float32)
+    x[t // 2, 5] = float("inf")
+    y = ops.mx4_mul_mat(pack(code, e), x).cpu().numpy()
+    nan = np.zeros((t, m), bool)
+    nan[t // 2] = nan[:, m // 2] = True
+    assert (np.isnan(y) == nan).all()
+    x64[t // 2] = 0
+    e[m // 2, -1] = 0
+    want = np_rounded(x64) @ np_values(code, e).T
+    assert np.abs(np.where(nan, 0, y - want)).max() <= 1e-4 * np.abs(want).max()
+
+
+@gpu
+def test_product_extreme_exponents():
+    """Exponents that cancel: 2^120 times 2^-120; both so small that the result is zero."""
+    code = np.full((4, 64), 2, np.uint8)   # ones
+    one = lambda b: (code, np.full((4, 2), b, np.uint8))  # noqa: E731
+    big, small = one(247), one(7)
+    y = ops.mx4_mul_mat(pack(*big), pack(*small), torch.float32)
+    assert (y == 64).all()
+    assert (ops.mx4_mul_mat(pack(*small), pack(*small), torch.float32) == 0).all()
+    assert (ops.mx4_mul_mat(pack(*big), pack(*big), torch.float32) == float("inf")).all()
+
+
+# ---- routing -------------------------------------------------------------------------------------
+SORTS = [(1, 1, 1), (1, 2, 8), (3, 2, 8), (7, 16, 5), (64, 1, 64), (65, 3, 33), (1000, 4, 256), (511, 8, 1024), (2048, 2, 7),
+         (5000, 2, 100), (40000, 4, 1000), (140000, 4, 9)]
+
+
+@gpu
+@pytest.mark.parametrize("t,used,n_expert", SORTS)
+@pytest.mark.parametrize("kind", ["even", "holes", "one", "none"])
+def test_sort(t, used, n_expert, kind):
+    rng = np.random.default_rng(t)
+    ids = routing(rng, t, used, n_expert, kind)
+    want = np_sort(ids, n_expert)
+    for dtype in (torch.int32, torch.int64):
+        plan = ops.moe_sort(torch.from_numpy(ids).to(dtype).cuda(), n_expert)
+        for got, w in zip(plan, want):
+            assert got.dtype == torch.int32 and (got.cpu().numpy() == w).all()
+
+
+@gpu
+def test_sort_of_wide_ids_and_no_tokens():
+    ids = torch.tensor([[1 << 32, 1], [-(1 << 32), (1 << 32) + 1]]).cuda()
+    plan = ops.moe_sort(ids, 2)
+    assert plan.rank.tolist() == [[-1, 0], [-1, -1]] and plan.offsets.tolist() == [0, 0, 1] and plan.order.tolist() == [1, -1, -1, -1]
+    plan = ops.moe_sort(ids[:0], 3)
+    assert plan.offsets.tolist() == [0, 0, 0, 0] and plan.order.numel() == 0
+    assert ops.moe_gather(torch.zeros(0, 8, device="cuda"), plan).shape == (0, 8)
+    assert ops.moe_combine(torch.zeros(0, 8, device="cuda"), plan).shape == (0, 8)
+
+
+ROWS = [(1, 1, 3, 1), (1, 2, 8, 4096), (5, 3, 4, 33), (9, 2, 6, 34), (17, 16, 9, 36), (40, 8, 128, 2048), (130, 1, 3, 257), (300, 4, 8, 1000)]
+
+
+def plan_of(rng, t, used, n_expert, kind):
+    ids = routing(rng, t, used, n_expert, kind)
+    order, rank, offsets = np_sort(ids, n_expert)
+    return ids, order, rank, ops.MoePlan(*(torch.from_numpy(v).cuda() for v in (order, rank, offsets)))
+
+
+@gpu
+@pytest.mark.parametrize("t,used,n_expert,d", ROWS)
+@pytest.mark.parametrize("kind", ["even", "holes", "none"])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gather_combine_and_gradients(t, used, n_expert, d, kind, dtype):
+    rng = np.random.default_rng(t * d)
+    ids, order, rank, plan = plan_of(rng, t, used, n_expert, kind)
+    held = int((order >= 0).sum())
+    x, x64 = rows_of(rng, t, d, dtype)
+    xs = ops.moe_gather(x, plan).double().cpu().numpy()
+    assert (xs[:held] == x64[order[:held] // used]).all() and (xs[held:] == 0).all()
+
+    ys, ys64 = rows_of(rng, t * used, d, dtype)
+    ys[held:] = float("nan")        # rows and weights of slots without an expert are not looked at
+    w = torch.from_numpy(rng.random((t, used), dtype=np.float32)).cuda()
+    w[torch.from_numpy(rank < 0).cuda()] = float("inf")
+    w64 = np.where(rank < 0, 0, w.double().cpu().numpy())
+    rows = np.where((rank >= 0)[..., None], ys64[np.maximum(rank, 0)], 0)
+    for weights, f in ((w, w64), (None, np.ones((t, used)))):
+        got = ops.moe_combine(ys, plan, weights).double().cpu().numpy()
+        want, room = (rows * f[..., None]).sum(1), np.abs(rows * f[..., None]).sum(1) * 2 * used * U32
+        assert (np.abs(got - want) <= room + half_step(dtype) * (np.abs(want) + room) + least_step(dtype)).all()
+
+    dy, dy64 = rows_of(rng, t, d, dtype)
+    dys, dw = ops.moe_combine_back(dy, ys, plan, w)
+    want = np.zeros((t * used, d))
+    want[:held] = w64.reshape(-1)[order[:held], None] * dy64[order[:held] // used]
+    got = dys.double().cpu().numpy()
+    assert (np.abs(got - want) <= (U32 + half_step(dtype) * (1 + U32)) * np.abs(want) + least_step(dtype)).all() and (got[held:] == 0).all()
+    want, room = (rows * dy64[:, None]).sum(-1), np.abs(rows * dy64[:, None]).sum(-1) * (d + 1) * U32
+    assert (np.abs(dw.double().cpu().numpy() - want) <= room).all()
+
+
+@gpu
+def test_gradients_against_differences():
+    """y is linear in the rows and in the weights: differences of the combine itself, taken in steps of
+    powers of two on small whole numbers, are exact."""
+    rng = np.random.default_rng(11)
+    _, _, rank, plan = plan_of(rng, 6, 3, 4, "holes")
+    ys = torch.from_numpy(rng.integers(-8, 9, (18, 5)).astype(np.float32)).cuda()
+    w = torch.from_numpy(rng.integers(-8, 9, (6, 3)).astype(np.float32)).cuda()
+    dy = torch.from_numpy(rng.integers(-8, 9, (6, 5)).astype(np.float32)).cuda()
+    dys, dw = ops.moe_combine_back(dy, ys, plan, w)
+    loss = lambda a, b: float((ops.moe_combine(a, plan, b) * dy).sum())  # noqa: E731
+    base = loss(ys, w)
+    for i in range(18):
+        for j in range(5):
+            a = ys.clone()
+            a[i, j] += 2
+            assert loss(a, w) - base == 2 * float(dys[i, j])
+    for i in range(6):
+        for j in range(3):
+            b = w.clone()
+            b[i, j] += 2
+            assert loss(ys, b) - base == 2 * float(dw[i, j])
+    x = torch.from_numpy(rng.integers(-8, 9, (6, 5)).astype(np.float32)).cuda()
+    dx = ops.moe_combine(dys, plan)     # the gather's gradient for a loss of xs . dys
+    for i in range(6):
+        for j in range(5):
+            a = x.clone()
+            a[i, j] += 1
+            assert float(((ops.moe_gather(a, plan) - ops.moe_gather(x, plan)) * dys).sum()) == float(dx[i, j])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strided_rows_of_the_routing(dtype):
+    rng = np.random.default_rng(2)
+    _, _, _, plan = plan_of(rng, 10, 2, 4, "holes")
+    big, _ = rows_of(rng, 40, 90, dtype)
+    w = torch.rand(10, 2, device="cuda")
+    for first, d in ((0, 64), (1, 64), (2, 33), (8, 72)):
+        x, ys = big[:20:2, first:first + d], big[::2, first:first + d]
+        assert torch.equal(ops.moe_gather(x, plan), ops.moe_gather(x.contiguous(), plan))
+        assert torch.equal(ops.moe_combine(ys, plan, w), ops.moe_combine(ys.contiguous(), plan, w))
+        for a, b in zip(ops.moe_combine_back(x, ys, plan, w), ops.moe_combine_back(x.contiguous(), ys.contiguous(), plan, w)):
+            assert torch.equal(a, b)
+
+
+# ---- the experts' product ------------------------------------------------------------------------
+EXPERTS = [(1, 2, 8, 48, 64), (1, 1, 1, 16, 32), (3, 2, 8, 33, 288), (20, 6, 64, 40, 160), (37, 2, 3, 130, 512), (100, 4, 100, 17, 96),
+           (200, 2, 4, 300, 320), (700, 1, 2, 257, 288), (90, 8, 300, 64, 256)]
+
+
+@gpu
+@pytest.mark.parametrize("t,used,n_expert,m,k", EXPERTS)
+@pytest.mark.parametrize("kind", ["even", "holes", "one", "none"])
+@pytest.mark.parametrize("sorted_rows", [False, True])
+def test_experts_product(t, used, n_expert, m, k, kind, sorted_rows):
+    rng = np.random.default_rng(t + m)
+    dtype = TYPES[(t + m + sorted_rows) % 3]
+    ids, order, rank, plan = plan_of(rng, t, used, n_expert, kind)
+    held = int((order >= 0).sum())
+    w, w64 = random_mx4(rng, n_expert, m, k)
+    x, x64 = rows_of(rng, t * used if sorted_rows else t, k, dtype)
+    if sorted_rows:
+        x[held:] = float("nan")     # rows that no expert takes are not looked at
+    y = ops.mx4_mul_mat_id(w, x, plan, x_sorted=sorted_rows)
+    assert y.dtype == dtype and y.shape == (t * used, m) and (y[held:] == 0).all()
+    xr = np_rounded(x64)
+    flat = ids.reshape(-1)
+    for e in range(n_expert):
+        at = np.flatnonzero(flat[order[:held]] == e)
+        rows = at if sorted_rows else order[at] // used
+        check_product(y[torch.from_numpy(at).cuda()], w64[e], xr[rows], dtype, f"expert {e}")
+    assert torch.equal(ops.mx4_mul_mat_id(w, ops.mx4_quantize(x), plan, sorted_rows, dtype), y)
+
+
+# ---- together ------------------------------------------------------------------------------------
+def expert_layer(x, ids, weights, up, down, n_expert):
+    plan = ops.moe_sort(ids, n_expert)
+    h = ops.mx4_mul_mat_id(up, x, plan)
+    f = h.shape[1] // 2
+    h = torch.nn.functional.silu(h[:, :f]) * h[:, f:]
+    return ops.moe_combine(ops.mx4_mul_mat_id(down, h, plan, x_sorted=True), plan, weights)
+
+
+def layer_case(t, seed=1, n_expert=8, used=2, d=512, f=288):
+    rng = np.random.default_rng(seed)
+    up, up64 = random_mx4(rng, n_expert, 2 * f, d)
+    down, down64 = random_mx4(rng, n_expert, d, f)
+    x, x64 = rows_of(rng, t, d, torch.float32)
+    logits = torch.from_numpy(rng.standard_normal((t, n_expert))).float().cuda()
+    weights, ids = torch.topk(torch.softmax(logits, 1), used)
+    return (x, ids, weights, up, down, n_expert), (x64, up64, down64)
+
+
+@gpu
+@pytest.mark.parametrize("t", [1, 4, 50, 300])
+def test_expert_layer(t):
+    """A layer of experts as a model runs it.  The second quantisation rounds what the first product
+    left off by float32 sums, so an activation next to a border may fall to either side: the second
+    product is checked from the activations that the framework computed."""
+    args, (x64, up64, down64) = layer_case(t)
+    x, ids, weights, up, down, n_expert = args
+    y = expert_layer(*args)
+    plan = ops.moe_sort(ids, n_expert)
+    h = ops.mx4_mul_mat_id(up, x, plan)
+    f = h.shape[1] // 2
+    a = torch.nn.functional.silu(h[:, :f]) * h[:, f:]
+    ids, rank, w64 = ids.cpu().numpy(), plan.rank.cpu().numpy(), weights.double().cpu().numpy()
+    xr, ar = np_rounded(x64), np_rounded(a.double().cpu().numpy())
+    want, room = np.zeros_like(x64), np.zeros_like(x64)
+    for i in range(t):
+        for j in range(2):
+            e, p = ids[i, j], rank[i, j]
+            check_product(h[p][None], up64[e], xr[i][None], torch.float32)
+            one, size = down64[e] @ ar[p], np.abs(down64[e]) @ np.abs(ar[p])
+            want[i] += w64[i, j] * one
+            room[i] += w64[i, j] * size * (ar.shape[1] + 5) * U32
+    assert (np.abs(y.double().cpu().numpy() - want) <= room).all()
+
+
+@gpu
+@pytest.mark.parametrize("t", [1, 40])
+def test_expert_layer_in_a_graph(t):
+    """Captured once, replayed on new inputs with eager work between; the eager calls agree bit for bit."""
+    args, _ = layer_case(t)
+    x, ids, weights = (v.clone() for v in args[:3])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        expert_layer(x, ids, weights, *args[3:])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = expert_layer(x, ids, weights, *args[3:])
+    for seed in range(4):
+        fresh, _ = layer_case(t, seed)
+        for to, src in zip((x, ids, weights), fresh[:3]):
+            to.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, expert_layer(x, ids, weights, *args[3:]))
+
+
+@gpu
+def test_streams_and_repeatability():
+    args, _ = layer_case(64)
+    want = expert_layer(*args)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            got.append([expert_layer(*args) for _ in range(5)])
+    torch.cuda.synchronize()
+    assert all(torch.equal(want, y) for ys in got for y in ys)
+
+
+@gpu
+def test_flat_abi_on_a_private_stream():
+    """stream NULL: done when the call returns."""
+    rng = np.random.default_rng(0)
+    x, x64 = rows_of(rng, 4, 64, torch.float32)
+    codes, scales = torch.empty(4, 32, dtype=torch.uint8, device="cuda"), torch.empty(1, 4, 8, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    assert ops.library().mi355x_mx4_quantize(0, x.data_ptr(), 64, 4, 64, codes.data_ptr(), scales.data_ptr(), None) == 0
+    code, e = unpack(ops.Mx4(codes, scales))
+    assert (code == np_quantize(x64)[0]).all() and (e == np_quantize(x64)[1]).all()
+
+
+@gpu
+def test_tensors_refused_on_the_host():
+    rng = np.random.default_rng(0)
+    x = torch.zeros(4, 64, device="cuda")
+    w, _ = random_mx4(rng, 8, 64)
+    we, _ = random_mx4(rng, 3, 8, 64)
+    _, _, _, plan = plan_of(rng, 4, 2, 3, "even")
+    rows, weights = torch.zeros(8, 64, device="cuda"), torch.zeros(4, 2, device="cuda")
+    bad = [
+        (ValueError, lambda: ops.mx4_quantize(x[:, :40])), (ValueError, lambda: ops.mx4_quantize(x[0])),
+        (TypeError, lambda: ops.mx4_quantize(x.double())), (ValueError, lambda: ops.mx4_quantize(torch.zeros(64, 4, device="cuda").t())),
+        (ValueError, lambda: ops.mx4_quantize(x.expand(4, 64)[:1].expand(4, 64))), (ValueError, lambda: ops.mx4_quantize(x.clone().requires_grad_())),
+        (TypeError, lambda: ops.mx4_dequantize(w, torch.int32)), (ValueError, lambda: ops.mx4_dequantize(we)),
+        (ValueError, lambda: ops.mx4_dequantize(ops.Mx4(w.codes[:, :24], w.scales))),
+        (ValueError, lambda: ops.mx4_dequantize(ops.Mx4(w.codes, w.scales[:, :7]))),
+        (TypeError, lambda: ops.mx4_dequantize(ops.Mx4(w.codes.to(torch.int8), w.scales))),
+        (ValueError, lambda: ops.mx4_mul_mat(w, x[:, :32])), (TypeError, lambda: ops.mx4_mul_mat(w, x.long())),
+        (TypeError, lambda: ops.mx4_mul_mat(w, x, torch.float64)), (ValueError, lambda: ops.mx4_mul_mat(we, x)),
+        (ValueError, lambda: ops.mx4_mul_mat_id(we, x[:3], plan)), (ValueError, lambda: ops.mx4_mul_mat_id(we, x, plan, x_sorted=True)),
+        (ValueError, lambda: ops.mx4_mul_mat_id(ops.Mx4(we.codes[:2], we.scales[:2]), x, plan)),
+        (TypeError, lambda: ops.mx4_mul_mat_id(we, x, tuple(plan))),
+        (TypeError, lambda: ops.moe_sort(weights, 3)), (ValueError, lambda: ops.moe_sort(plan.rank, 0)),
+        (ValueError, lambda: ops.moe_sort(plan.rank, 1025)), (ValueError, lambda: ops.moe_sort(plan.rank.t(), 3)),
+        (ValueError, lambda: ops.moe_sort(torch.zeros(2, 17, dtype=torch.int32, device="cuda"), 3)),
+        (ValueError, lambda: ops.moe_gather(rows, plan)), (ValueError, lambda: ops.moe_combine(x, plan, weights)),
+        (ValueError, lambda: ops.moe_combine(rows, plan, weights[:3])), (TypeError, lambda: ops.moe_combine(rows, plan, weights.half())),
+        (TypeError, lambda: ops.moe_combine(rows, plan._replace(order=plan.order.long()), weights)),
+        (ValueError, lambda: ops.moe_combine(rows, plan._replace(order=plan.order[:4]), weights)),
+        (TypeError, lambda: ops.moe_combine_back(x.half(), rows, plan, weights)), (ValueError, lambda: ops.moe_combine_back(x[:3], rows, plan, weights)),
+        (ValueError, lambda: ops.moe_combine_back(x, rows, plan, weights.clone().requires_grad_())),
+    ]
+    for i, (kind, call) in enumerate(bad):
+        with pytest.raises(kind):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    with torch.no_grad():
+        ops.mx4_quantize(x.clone().requires_grad_())
