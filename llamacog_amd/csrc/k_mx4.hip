@@ -211,6 +211,7 @@ static mx4_args product_args(const mx4_mat & w, const mx4_mat & x, void * y) {
 
 hipError_t mx4_product(const mx4_mat & w, const mx4_mat & x, int ytype, void * y, hipStream_t st) {
     const mx4_args a = product_args(w, x, y);
+    if (x.rows > 64) return mx4_product_tile(a, ytype, st);
     return product_mv<false>(a, x.rows, ytype, st);
 }
 
@@ -221,6 +222,7 @@ hipError_t mx4_product_id(const mx4_mat & w, const mx4_mat & x, const moe_view &
     a.n_expert = v.n_expert;
     a.used = v.used;
     a.T = v.pairs;
+    if (v.pairs > 64 * v.n_expert) return mx4_product_tile(a, ytype, st);
     return product_mv<true>(a, v.pairs, ytype, st);
 }
 

@@ -107,6 +107,8 @@ struct mx4_args {
     void * y;
 };
 
+hipError_t mx4_product_tile(const mx4_args & a, int ytype, hipStream_t st);   // k_mx4_gemm.hip; by experts with a.offsets
+
 // ---- tiles of sorted pairs -------------------------------------------------------------------
 struct tile_rows {
     int64_t expert;   // -1: rows behind the last expert's
