@@ -79,37 +79,26 @@ static __device__ __forceinline__ void mma_step(v16f (&acc)[FM][FN], const frags
 // Workgroup -> tile.  Consecutive workgroups go round the eight XCDs: each XCD gets one run of the
 // tiles, so that what its workgroups share meets in its L2.  A run goes along GROUP x tiles, then
 // to the next weight tile: the 32 that an XCD has at a time are about 4 by 8.
-static __device__ __forceinline__ void tile_of(int64_t id, int64_t tiles_m, int64_t tiles_n, int64_t & tm, int64_t & tn) {
-    constexpr int GROUP = 8;
-    const int64_t n = tiles_m * tiles_n, xcd = id & 7;
+static __device__ __forceinline__ void tile_of(unsigned id, unsigned tiles_m, unsigned tiles_n, unsigned & tm, unsigned & tn) {
+    constexpr unsigned GROUP = 8;
+    const unsigned n = tiles_m * tiles_n, xcd = id & 7;
     id = xcd * (n >> 3) + min(xcd, n & 7) + (id >> 3);
-    const int64_t g = id / (GROUP * tiles_m), wide = min((int64_t) GROUP, tiles_n - g * GROUP);
+    const unsigned g = id / (GROUP * tiles_m), wide = min(GROUP, tiles_n - g * GROUP);
     id -= g * GROUP * tiles_m;
     tm = id / wide;
     tn = g * GROUP + id % wide;
 }
 
-template <class Y, int N> static __device__ __forceinline__ void store_out(Y * y, const float * v, int64_t left) {
-    if (left >= N) {
-        pack<Y, N> q;
-#pragma unroll
-        for (int i = 0; i < N; ++i) q.v[i] = from_f32<Y>(v[i]);
-        *(pack<Y, N> *) y = q;
-    } else {
-        for (int i = 0; i < left; ++i) y[i] = from_f32<Y>(v[i]);
-    }
-}
-
 template <int FM, int FN, int WM, int WN, class Y, bool IDS>
-static __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tile(mx4_args a, int64_t tiles_m, int64_t tiles_n) {
+static __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tile(mx4_args a, unsigned tiles_m, unsigned tiles_n) {
     using S = tile_shape<FM, FN, WM, WN>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int64_t tm, tn;
+    unsigned tm, tn;
     tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
-    const int64_t m0 = tm * S::TM;
-    const tile_rows tr = IDS ? find_tile(a, tn, S::TN) : tile_rows{0, tn * S::TN, min((int64_t) S::TN, a.T - tn * S::TN)};
+    const int64_t m0 = (int64_t) tm * S::TM;
+    const tile_rows tr = IDS ? find_tile(a, tn, S::TN) : tile_rows{0, (int64_t) tn * S::TN, min((int64_t) S::TN, a.T - (int64_t) tn * S::TN)};
     if (tr.n <= 0) return;
     Y * y = (Y *) a.y;
     if (IDS && tr.expert < 0) {   // pairs that no expert takes
@@ -224,38 +213,63 @@ static __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tile(mx4_args a, in
     mma_step<2>(acc, f0, sa, sb, [&](auto i) { reads(f1, at, 3, i); });
     mma_step<3>(acc, f1, sa, sb, [](auto) {});
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no copy is left when the shared memory is given back
-    const bool wide = a.M % 4 == 0;
+
+    // The results go out through shared memory: straight from the registers a store would touch 32 x
+    // rows with 16 bytes each.  Rows of TM outputs lie 16 B past a multiple of the 64 banks apart, so
+    // that 16 x rows times four neighbouring outputs cover them.
+    constexpr int ROW = S::TM * (int) sizeof(Y) + 16;
+    constexpr int PASSES = (S::TN * ROW + 2 * S::STAGE - 1) / (2 * S::STAGE), PT = S::TN / PASSES;
+    static_assert(PT % 32 == 0 && PT * ROW <= 2 * S::STAGE, "whole fragments in a pass");
+    const int cols = (int) min((int64_t) S::TM, a.M - m0);
+    const bool wide = a.M * (int64_t) sizeof(Y) % 16 == 0;
+    Y * out = y + tr.first * a.M + m0;
 #pragma unroll
-    for (int n = 0; n < FN; ++n) {
-        const int64_t t = wn - S::TM + n * 32 + r31;
-        if (t >= tr.n) continue;
+    for (int pass = 0; pass < PASSES; ++pass) {
+        __syncthreads();
 #pragma unroll
-        for (int m = 0; m < FM; ++m)
+        for (int n = 0; n < FN; ++n) {
+            const int t = wn - S::TM + n * 32 - pass * PT;
+            if (t < 0 || t >= PT) continue;
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const int64_t row = m0 + wm + m * 32 + 2 * i + 4 * (lane >> 5);
-                float v[4] = {acc[m][n][i], acc[m][n][i + 1], acc[m][n][i + 2], acc[m][n][i + 3]};
-                Y * to = y + (tr.first + t) * a.M + row;
-                if (wide) {
-                    if (row < a.M) store_out<Y, 4>(to, v, 4);
-                } else {
-                    for (int k = 0; k < 4; ++k)
-                        if (row + k < a.M) to[k] = from_f32<Y>(v[k]);
+            for (int m = 0; m < FM; ++m)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    pack<Y, 4> q;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) q.v[k] = from_f32<Y>(acc[m][n][i + k]);
+                    *(pack<Y, 4> *) (lds + (t + r31) * ROW + (wm + m * 32 + 2 * i + 4 * half) * sizeof(Y)) = q;
                 }
-            }
+        }
+        __syncthreads();
+        const int rows = (int) min((int64_t) PT, tr.n - pass * PT);
+        if (wide) {
+            constexpr int V = 16 / sizeof(Y), PER = S::TM / V;
+            for (int i = threadIdx.x; i < rows * PER; i += 64 * S::NW)
+                if (i % PER * V < cols)
+                    *(pack<Y, V> *) (out + (int64_t) (pass * PT + i / PER) * a.M + i % PER * V) =
+                        *(const pack<Y, V> *) (lds + i / PER * ROW + i % PER * 16);
+        } else {
+            for (int i = threadIdx.x; i < rows * S::TM; i += 64 * S::NW)
+                if (i % S::TM < cols)
+                    out[(int64_t) (pass * PT + i / S::TM) * a.M + i % S::TM] =
+                        *(const Y *) (lds + i / S::TM * ROW + i % S::TM * (int) sizeof(Y));
+        }
     }
 }
+
+constexpr int64_t MAX_GROUPS = ((int64_t) 1 << 32) / 64 - 1;   // waves of a launch: its threads are counted in 32 bits
 
 template <int FM, int FN, int WM, int WN, bool IDS>
 static hipError_t run_tile(const mx4_args & a, int ytype, hipStream_t st) {
     using S = tile_shape<FM, FN, WM, WN>;
     const int64_t tm = (a.M + S::TM - 1) / S::TM, tn = IDS ? id_tiles(a, S::TN) : (a.T + S::TN - 1) / S::TN;
+    if (tm * tn > MAX_GROUPS / S::NW) return hipErrorInvalidConfiguration;
     return with_type(ytype, [&](auto t) {
         using Y = decltype(t);
         auto * k = k_mx4_tile<FM, FN, WM, WN, Y, IDS>;
         const hipError_t e = hipFuncSetAttribute((const void *) k, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * S::STAGE);
         if (e != hipSuccess) return e;
-        k<<<(unsigned) (tm * tn), 64 * S::NW, 2 * S::STAGE, st>>>(a, tm, tn);
+        k<<<(unsigned) (tm * tn), 64 * S::NW, 2 * S::STAGE, st>>>(a, (unsigned) tm, (unsigned) tn);
         return hipGetLastError();
     });
 }
