@@ -124,7 +124,7 @@ def routing(rng, t, used, n_expert, kind):
 def test_library_exports_what_the_header_declares():
     text = re.sub(r"//.*", "", open(os.path.join(la.REPO, "include", "ggml-mi355x.h")).read())
     names = set(re.findall(r"\bmi355x_(?:mx4|moe)_\w+(?=\s*\()", text))
-    assert names == {n for n in ops._SIGNATURES}
+    assert names == set(SIGNATURES)
     out = subprocess.run(["nm", "-D", "--defined-only", ops.LIBRARY], capture_output=True, text=True, check=True).stdout
     exported = {line.split()[-1] for line in out.splitlines() if " T " in line}
     assert exported == names   # nothing else, so that the plugin's copy of the kernels stays apart
@@ -137,6 +137,28 @@ def test_header_stands_alone(tmp_path, compiler, language):
     src.write_text('#include "ggml-mi355x.h"\nint main(void) { return mi355x_moe_sort_workspace(1, 1, 1) != 0; }\n')
     subprocess.run([compiler, "-x", language, "-Wall", "-Werror", "-fsyntax-only", "-I", os.path.join(la.REPO, "include"), str(src)],
                    check=True)
+
+
+P, I, L = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64
+SIGNATURES = {
+    "mi355x_mx4_quantize": [I, P, L, L, L, P, P, P],
+    "mi355x_mx4_dequantize": [P, P, L, L, I, P, P],
+    "mi355x_mx4_mul_mat": [P, P, L, L, I, P, P, L, L, I, P, P, L, P],
+    "mi355x_mx4_mul_mat_id": [P, P, L, L, L, I, P, P, L, L, L, I, P, P, I, P, P, L, P],
+    "mi355x_moe_sort": [P, I, L, L, L, P, P, P, P, L, P],
+    "mi355x_moe_gather": [I, P, L, L, L, L, P, P, P, P],
+    "mi355x_moe_combine": [I, P, L, L, L, L, P, P, P, P],
+    "mi355x_moe_combine_back": [I, P, L, P, L, L, L, L, P, P, P, P, P, P],
+    "mi355x_mx4_scales_bytes": [L, L],
+    "mi355x_mx4_mul_mat_workspace": [L, L],
+    "mi355x_moe_sort_workspace": [L, L, L],
+}
+
+
+def flat(name):
+    f = getattr(ops.library(), name)
+    f.argtypes, f.restype = SIGNATURES[name], L if name.endswith(("_bytes", "_workspace")) else I
+    return f
 
 
 A = 1 << 20   # an aligned address that no call below gets to read
@@ -183,7 +205,7 @@ REFUSED = [
 
 @pytest.mark.parametrize("name,args,code", REFUSED, ids=[f"{n[7:]}-{i}" for i, (n, _, _) in enumerate(REFUSED)])
 def test_flat_calls_refused_before_any_launch(name, args, code):
-    assert getattr(ops.library(), name)(*args, None) == code
+    assert flat(name)(*args, None) == code
 
 
 EMPTY = [
@@ -200,15 +222,14 @@ EMPTY = [
 
 @pytest.mark.parametrize("name,args", EMPTY, ids=[f"{n[7:]}-{i}" for i, (n, _) in enumerate(EMPTY)])
 def test_flat_calls_with_nothing_to_do(name, args):
-    assert getattr(ops.library(), name)(*args, None) == 0
+    assert flat(name)(*args, None) == 0
 
 
 def test_sizes():
-    lib = ops.library()
-    assert lib.mi355x_mx4_scales_bytes(3, 288) == 2 * 3 * 8 and lib.mi355x_mx4_scales_bytes(3, 289) == -1
-    assert lib.mi355x_mx4_mul_mat_workspace(3, 288) == 512 + 48
-    assert lib.mi355x_moe_sort_workspace(10, 2, 8) == 0 and lib.mi355x_moe_sort_workspace(1, 17, 8) == -1
-    assert lib.mi355x_moe_sort_workspace(1 << 20, 2, 8) > 0
+    scales, work, sort = flat("mi355x_mx4_scales_bytes"), flat("mi355x_mx4_mul_mat_workspace"), flat("mi355x_moe_sort_workspace")
+    assert scales(3, 288) == 2 * 3 * 8 and scales(3, 289) == -1
+    assert work(3, 288) == 512 + 48 and work(3, 0) == -1
+    assert sort(10, 2, 8) == 0 and sort(1, 17, 8) == -1 and sort(1 << 20, 2, 8) > 0
 
 
 def test_tensors_of_the_host_are_refused():
@@ -575,7 +596,7 @@ def test_flat_abi_on_a_private_stream():
     x, x64 = rows_of(rng, 4, 64, torch.float32)
     codes, scales = torch.empty(4, 32, dtype=torch.uint8, device="cuda"), torch.empty(1, 4, 8, dtype=torch.uint8, device="cuda")
     torch.cuda.synchronize()
-    assert ops.library().mi355x_mx4_quantize(0, x.data_ptr(), 64, 4, 64, codes.data_ptr(), scales.data_ptr(), None) == 0
+    assert flat("mi355x_mx4_quantize")(0, x.data_ptr(), 64, 4, 64, codes.data_ptr(), scales.data_ptr(), None) == 0
     code, e = unpack(ops.Mx4(codes, scales))
     assert (code == np_quantize(x64)[0]).all() and (e == np_quantize(x64)[1]).all()
 
