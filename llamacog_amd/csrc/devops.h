@@ -47,6 +47,10 @@ hipError_t mx4_dequantize(const mx4_mat & m, int type, void * y, hipStream_t st)
 hipError_t mx4_product(const mx4_mat & w, const mx4_mat & x, int ytype, void * y, hipStream_t st);
 // y [pairs][M]: sorted row p is expert e(p)'s W times x row order[p] / used (or p)
 hipError_t mx4_product_id(const mx4_mat & w, const mx4_mat & x, const moe_view & v, int ytype, void * y, hipStream_t st);
+// few rows of floats, quantised where they are used: whether that is the way for them, and the product
+bool mx4_takes_floats(const mx4_mat & w, int64_t x_rows, const moe_view * v);
+hipError_t mx4_product_float(const mx4_mat & w, int xtype, const void * x, int64_t ldx, int64_t x_rows, const moe_view * v,
+                             int ytype, void * y, hipStream_t st);
 
 size_t moe_sort_workspace(int64_t pairs, int n_expert);
 hipError_t moe_sort(const void * ids, int id_bytes, int64_t pairs, int n_expert, int32_t * order, int32_t * rank,

@@ -111,7 +111,7 @@ OPS_API int64_t mi355x_mx4_mul_mat_workspace(int64_t T, int64_t K) {
 
 // the x operand of a product: MXFP4 as given, or quantised into the workspace
 static int x_operand(int xtype, const void * x, const uint8_t * xscales, int64_t ldx, int64_t rows, int64_t K, void * work,
-                     int64_t work_bytes, hipStream_t st, mx4_mat & m) {
+                     hipStream_t st, mx4_mat & m) {
     if (xtype == MI355X_MX4) {
         m = {(const uint8_t *) x, xscales, rows, K};
         return 0;
@@ -141,9 +141,12 @@ OPS_API int mi355x_mx4_mul_mat(const uint8_t * w_codes, const uint8_t * w_scales
     if (T == 0 || M == 0) return 0;
     call_stream cs(stream);
     if (cs.err != hipSuccess) return MI355X_ERR_HIP;
+    const mx4_mat w = {w_codes, w_scales, M, K};
+    if (xtype != MI355X_MX4 && mx4_takes_floats(w, T, nullptr))
+        return cs.done(mx4_product_float(w, xtype, x, ldx, T, nullptr, ytype, y, cs.st));
     mx4_mat xm;
-    TRY(x_operand(xtype, x, x_scales, ldx, T, K, work, work_bytes, cs.st, xm));
-    return cs.done(mx4_product({w_codes, w_scales, M, K}, xm, ytype, y, cs.st));
+    TRY(x_operand(xtype, x, x_scales, ldx, T, K, work, cs.st, xm));
+    return cs.done(mx4_product(w, xm, ytype, y, cs.st));
 }
 
 OPS_API int mi355x_mx4_mul_mat_id(const uint8_t * w_codes, const uint8_t * w_scales, int64_t M, int64_t K, int64_t n_expert,
@@ -160,10 +163,13 @@ OPS_API int mi355x_mx4_mul_mat_id(const uint8_t * w_codes, const uint8_t * w_sca
     if (T == 0 || M == 0) return 0;
     call_stream cs(stream);
     if (cs.err != hipSuccess) return MI355X_ERR_HIP;
-    mx4_mat xm;
-    TRY(x_operand(xtype, x, x_scales, ldx, rows, K, work, work_bytes, cs.st, xm));
+    const mx4_mat w = {w_codes, w_scales, M, K};
     const moe_view v = {order, offsets, T * used, (int) n_expert, x_sorted ? 0 : (int) used};
-    return cs.done(mx4_product_id({w_codes, w_scales, M, K}, xm, v, ytype, y, cs.st));
+    if (xtype != MI355X_MX4 && mx4_takes_floats(w, rows, &v))
+        return cs.done(mx4_product_float(w, xtype, x, ldx, rows, &v, ytype, y, cs.st));
+    mx4_mat xm;
+    TRY(x_operand(xtype, x, x_scales, ldx, rows, K, work, cs.st, xm));
+    return cs.done(mx4_product_id(w, xm, v, ytype, y, cs.st));
 }
 
 OPS_API int64_t mi355x_moe_sort_workspace(int64_t T, int64_t used, int64_t n_expert) {

@@ -106,90 +106,180 @@ hipError_t mx4_dequantize(const mx4_mat & m, int type, void * y, hipStream_t st)
 }
 
 // ---- product, few rows -----------------------------------------------------------------------
-// A workgroup takes 16 weight rows and 16 NT x rows; its waves take the 256-element planes of K
-// in turn and their sums are joined in shared memory.  Weight rows are the matrix instruction's
-// first operand (16x16x128: lane l holds row l % 16 and the 32-block l / 16, one 16-B load), x rows
-// the second, so a lane's four results are four neighbouring outputs of one x row.
-template <int NT, int W, class Y, bool IDS>
-static __global__ void __launch_bounds__(64 * W) k_mx4_mv(mx4_args a) {
-    constexpr int U = NT == 1 ? 4 : 2;   // planes whose loads are issued together
-    __shared__ float red[W][NT][16][16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int r = lane & 15, q = lane >> 4;
-    const int64_t groups = (a.M + 15) / 16;
-    const int64_t m0 = (blockIdx.x % groups) * 16;
-    const int64_t tile = blockIdx.x / groups;
-    tile_rows tr = IDS ? find_tile(a, tile, 16 * NT) : tile_rows{0, tile * 16 * NT, min((int64_t) 16 * NT, a.T - tile * 16 * NT)};
+// Bound by the weights' bytes.  Weight rows are the matrix instruction's first operand (16x16x128:
+// lane l holds row l % 16 and the 32-block l / 16, one 16-B load; four lanes read 64 B of a row side
+// by side), x rows the second, so a lane's four results are four neighbouring outputs of an x row.
+//
+// A workgroup keeps the 16 NT x rows of a tile in shared memory and goes through groups of 16 weight
+// rows.  KS of its MV_WAVES waves share a group, each taking every KS-th 256-element plane of K, and
+// join their sums in shared memory; with KS = 1 there is nothing to join and no wave waits for
+// another.  KS is raised only where the groups alone are too few waves for the memory (mv_split).
+// A wave's next planes are always on their way while it multiplies the present ones.
+//
+// The x rows come as MXFP4, or as floats that every workgroup quantises for itself behind its first
+// weight loads: that costs a little arithmetic in each and saves a launch.
+constexpr int MV_WAVES = 8;
+
+// U planes of a row group
+template <int U> struct mv_weights {
+    int4 w[U][2];
+    uint2 e[U];
+    __device__ __forceinline__ void load(const mx4_args & a, const uint8_t * wc, const uint8_t * ws, int64_t row, int s0, int step, int q) {
+        const int S = (a.KB + 7) / 8;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int s = s0 + u * step;
+            if (s >= S) break;
+            e[u] = *(const uint2 *) (ws + ((int64_t) s * a.M + row) * 8);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) w[u][j] = *(const int4 *) (wc + (row * a.KB + min(s * 8 + 4 * j + q, a.KB - 1)) * 16);
+        }
+    }
+};
+
+struct mxfp4 {};   // the type of x rows that are quantised already
+
+template <int NT, int KS, class X, class Y, bool IDS>
+static __global__ void __launch_bounds__(64 * MV_WAVES, 4) k_mx4_mv(mx4_args a, const X * __restrict__ x, int64_t ldx, int per_tile) {
+    constexpr int U = 2, GW = MV_WAVES / KS;   // planes at a time; groups at a time
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // x rows, then sums to join
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, q = lane >> 4, part = wave % KS;
+    const int64_t tile = blockIdx.x / per_tile;
+    const tile_rows tr = IDS ? find_tile(a, tile, 16 * NT)
+                             : tile_rows{0, tile * 16 * NT, min((int64_t) 16 * NT, a.T - tile * 16 * NT)};
     if (tr.n <= 0) return;
-    Y * y = (Y *) a.y;
+    Y * y = (Y *) a.y + tr.first * a.M;
+    const int64_t g0 = blockIdx.x % per_tile * GW;
     if (IDS && tr.expert < 0) {   // pairs that no expert takes
-        for (int i = threadIdx.x; i < 16 * tr.n; i += 64 * W)
-            if (m0 + (i & 15) < a.M) y[(tr.first + (i >> 4)) * a.M + m0 + (i & 15)] = from_f32<Y>(0.0f);
+        for (int64_t g = g0; g * 16 < a.M; g += (int64_t) per_tile * GW)
+            for (int i = threadIdx.x; i < 16 * GW * tr.n; i += 64 * MV_WAVES) {
+                const int64_t m = g * 16 + i % (16 * GW);
+                if (m < a.M) y[i / (16 * GW) * a.M + m] = from_f32<Y>(0.0f);
+            }
         return;
     }
     const uint8_t * wc = a.w_codes + tr.expert * a.w_codes_stride;
     const uint8_t * ws = a.w_scales + tr.expert * a.w_scales_stride;
-    const int64_t row = min(m0 + r, a.M - 1);
-    const uint8_t * wrow = wc + row * (int64_t) a.KB * 16;
-    int64_t xr[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) xr[n] = x_row<IDS>(a, tr.first + min((int64_t) 16 * n + r, tr.n - 1));
     const int S = (a.KB + 7) / 8;
-    v4f acc[NT] = {};
-    for (int s0 = wave; s0 < S; s0 += W * U) {
-        int4 w[U][2], x[U][NT][2];
-        uint32_t sw[U][2], sx[U][NT][2];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int s = min(s0 + u * W, S - 1);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int64_t b = min(s * 8 + 4 * j + q, a.KB - 1);
-                w[u][j] = *(const int4 *) (wrow + b * 16);
-                sw[u][j] = *(const uint32_t *) (ws + ((int64_t) s * a.M + row) * 8 + 4 * j);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    x[u][n][j] = *(const int4 *) (a.x_codes + (xr[n] * a.KB + b) * 16);
-                    sx[u][n][j] = *(const uint32_t *) (a.x_scales + (s * a.x_rows + xr[n]) * 8 + 4 * j);
-                }
+    mv_weights<U> now, next;
+    auto row_of = [&](int64_t g) { return min((g + wave / KS) * 16 + r, a.M - 1); };
+    now.load(a, wc, ws, row_of(g0), part, KS, q);
+
+    const int row_bytes = mv_row_bytes(a.KB);
+    if constexpr (std::is_same_v<X, mxfp4>) {
+        for (int t = wave; t < tr.n; t += MV_WAVES) {
+            const int64_t row = x_row<IDS>(a, tr.first + t);
+            for (int c = lane; c < a.KB; c += 64) {
+                *(int4 *) (lds + t * row_bytes + c * 16) = *(const int4 *) (a.x_codes + (row * a.KB + c) * 16);
+                lds[t * row_bytes + a.KB * 16 + c] = a.x_scales[((c >> 3) * a.x_rows + row) * 8 + (c & 7)];
             }
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                // past K: zero codes and a finite exponent
-                const bool in = (s0 + u * W) * 8 + 4 * j + q < a.KB;
-                const int4 wv = in ? w[u][j] : int4{0, 0, 0, 0};
-                const int wsc = in ? (int) (sw[u][j] >> (8 * q)) : 0;
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const int xsc = in ? (int) (sx[u][n][j] >> (8 * q)) : 0;
-                    acc[n] = mfma_mx4_16(wv, x[u][n][j], acc[n], wsc, xsc);
-                }
+    } else {
+        const bool vec = (uintptr_t) x % 16 == 0 && ldx * (int64_t) sizeof(X) % 16 == 0;
+        for (int t = 0; t < tr.n; ++t) {
+            const X * row = x + x_row<IDS>(a, tr.first + t) * ldx;
+            for (int c = threadIdx.x; c < a.KB * 4; c += 64 * MV_WAVES) {
+                float v[8];
+                if (vec) load8<X, true>(row + (int64_t) c * 8, v);
+                else load8<X, false>(row + (int64_t) c * 8, v);
+                const unsigned e = mx4_block_exponent(v);
+                *(uint32_t *) (lds + t * row_bytes + c * 4) = mx4_pack8(v, e);
+                if ((c & 3) == 0) lds[t * row_bytes + a.KB * 16 + (c >> 2)] = (uint8_t) e;
             }
         }
     }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) *(v4f *) &red[wave][n][r][4 * q] = acc[n];
     __syncthreads();
-    for (int i = threadIdx.x; i < NT * 256; i += 64 * W) {
-        const int t = i >> 4, m = i & 15;
-        if (t >= tr.n || m0 + m >= a.M) continue;
-        float s = 0.0f;
+    const uint8_t * xl[NT];
 #pragma unroll
-        for (int k = 0; k < W; ++k) s += red[k][t >> 4][t & 15][m];
-        y[(tr.first + t) * a.M + m0 + m] = from_f32<Y>(s);
+    for (int n = 0; n < NT; ++n) xl[n] = lds + min(16 * n + r, (int) tr.n - 1) * row_bytes;
+    float * red = (float *) (lds + min((int64_t) 16 * NT, a.T) * row_bytes);   // [GW][KS][16 NT][16]
+
+    for (int64_t g = g0; g * 16 < a.M; g += (int64_t) per_tile * GW) {
+        v4f acc[NT] = {};
+        for (int s0 = part; s0 < S; s0 += KS * U) {
+            const bool more = s0 + KS * U < S;
+            next.load(a, wc, ws, row_of(more ? g : g + (int64_t) per_tile * GW), more ? s0 + KS * U : part, KS, q);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int s = s0 + u * KS;
+                if (s >= S) break;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int b = s * 8 + 4 * j + q, bc = min(b, a.KB - 1);
+                    const bool in = b < a.KB;   // past K: zero codes, finite exponents
+                    const int4 w = in ? now.w[u][j] : int4{0, 0, 0, 0};
+                    const int sw = in ? (int) ((j ? now.e[u].y : now.e[u].x) >> (8 * q)) : 0;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        acc[n] = mfma_mx4_16(w, *(const int4 *) (xl[n] + bc * 16), acc[n], sw, in ? xl[n][a.KB * 16 + bc] : 0);
+                }
+            }
+            now = next;
+        }
+        const int64_t m0 = (g + wave / KS) * 16;
+        if constexpr (KS == 1) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                if (16 * n + r < tr.n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (m0 + 4 * q + i < a.M) y[(16 * n + r) * a.M + m0 + 4 * q + i] = from_f32<Y>(acc[n][i]);
+        } else {
+            __syncthreads();   // the sums of the groups before have been taken
+#pragma unroll
+            for (int n = 0; n < NT; ++n) *(v4f *) &red[((wave * NT + n) * 16 + r) * 16 + 4 * q] = acc[n];
+            __syncthreads();
+            for (int i = threadIdx.x; i < GW * NT * 256; i += 64 * MV_WAVES) {
+                const int k = i / (NT * 256), t = i / 16 % (16 * NT);
+                const int64_t m = (g + k) * 16 + i % 16;
+                if (t >= tr.n || m >= a.M) continue;
+                float sum = 0.0f;
+#pragma unroll
+                for (int p = 0; p < KS; ++p) sum += red[(k * KS + p) * NT * 256 + i % (NT * 256)];
+                y[t * a.M + m] = from_f32<Y>(sum);
+            }
+        }
     }
 }
 
-template <bool IDS> static hipError_t product_mv(const mx4_args & a, int64_t tokens, int ytype, hipStream_t st) {
+constexpr int64_t MV_LDS = 144 * 1024;   // most shared memory of a workgroup
+
+static int64_t mv_lds(const mx4_args & a, int NT, int KS) {
+    return mv_row_bytes(a.KB) * (a.T < 16 * NT ? a.T : 16 * NT) + (KS > 1 ? MV_WAVES * NT * 1024 : 0);
+}
+
+// how many waves share a group of 16 weight rows: as few as give `tiles` tiles MV_FILL waves in all
+constexpr int64_t MV_FILL = 2048;
+static int mv_split(const mx4_args & a, int64_t tiles) {
+    const int64_t groups = (a.M + 15) / 16 * tiles;
+    int ks = 1;
+    while (ks < MV_WAVES && groups * ks < MV_FILL && a.KB > 8 * ks) ks *= 2;
+    return ks;
+}
+
+template <int NT, class X, bool IDS>
+static hipError_t run_mv(const mx4_args & a, const X * x, int64_t ldx, int ytype, hipStream_t st) {
+    const int64_t tiles = IDS ? id_tiles(a, 16 * NT) : (a.T + 16 * NT - 1) / (16 * NT);
+    const int64_t busy = IDS ? (a.T < a.n_expert ? a.T : a.n_expert) : tiles;   // tiles to reckon with
+    const int ks = mv_split(a, busy);
     return with_type(ytype, [&](auto t) {
         using Y = decltype(t);
-        const int64_t groups = (a.M + 15) / 16;
-        const int64_t tiles = IDS ? id_tiles(a, 16) : (tokens + 15) / 16;
-        k_mx4_mv<1, 4, Y, IDS><<<(unsigned) (groups * tiles), 256, 0, st>>>(a);
-        return hipGetLastError();
+        auto go = [&](auto split) {
+            constexpr int KS = split;
+            const int64_t rounds = ((a.M + 15) / 16 + MV_WAVES / KS - 1) / (MV_WAVES / KS);
+            const int64_t fair = (768 + busy - 1) / busy;   // three workgroups per CU in all, each with its turn of the groups
+            const int per_tile = (int) (rounds < fair ? rounds : fair);
+            if (per_tile * tiles > MAX_WAVES / MV_WAVES) return hipErrorInvalidConfiguration;
+            k_mx4_mv<NT, KS, X, Y, IDS><<<(unsigned) (per_tile * tiles), 64 * MV_WAVES, mv_lds(a, NT, KS), st>>>(a, x, ldx, per_tile);
+            return hipGetLastError();
+        };
+        switch (ks) {
+            case 1: return go(std::integral_constant<int, 1>{});
+            case 2: return go(std::integral_constant<int, 2>{});
+            case 4: return go(std::integral_constant<int, 4>{});
+            default: return go(std::integral_constant<int, 8>{});
+        }
     });
 }
 
@@ -209,6 +299,25 @@ static mx4_args product_args(const mx4_mat & w, const mx4_mat & x, void * y) {
     return a;
 }
 
+static mx4_args id_args(const mx4_mat & w, const mx4_mat & x, const moe_view & v, void * y) {
+    mx4_args a = product_args(w, x, y);
+    a.order = v.order;
+    a.offsets = v.offsets;
+    a.n_expert = v.n_expert;
+    a.used = v.used;
+    a.T = v.pairs;
+    return a;
+}
+
+// x rows of a tile: as many as shared memory holds, so that the weights are read once for all of them
+template <bool IDS> static hipError_t product_mv(const mx4_args & a, int64_t rows, int ytype, hipStream_t st) {
+    const mxfp4 * x = nullptr;
+    if (rows > 32 && mv_lds(a, 4, MV_WAVES) <= MV_LDS) return run_mv<4, mxfp4, IDS>(a, x, 0, ytype, st);
+    if (rows > 16 && mv_lds(a, 2, MV_WAVES) <= MV_LDS) return run_mv<2, mxfp4, IDS>(a, x, 0, ytype, st);
+    if (mv_lds(a, 1, MV_WAVES) <= MV_LDS) return run_mv<1, mxfp4, IDS>(a, x, 0, ytype, st);
+    return mx4_product_tile(a, ytype, st);
+}
+
 hipError_t mx4_product(const mx4_mat & w, const mx4_mat & x, int ytype, void * y, hipStream_t st) {
     const mx4_args a = product_args(w, x, y);
     if (x.rows > 64) return mx4_product_tile(a, ytype, st);
@@ -216,14 +325,27 @@ hipError_t mx4_product(const mx4_mat & w, const mx4_mat & x, int ytype, void * y
 }
 
 hipError_t mx4_product_id(const mx4_mat & w, const mx4_mat & x, const moe_view & v, int ytype, void * y, hipStream_t st) {
-    mx4_args a = product_args(w, x, y);
-    a.order = v.order;
-    a.offsets = v.offsets;
-    a.n_expert = v.n_expert;
-    a.used = v.used;
-    a.T = v.pairs;
+    const mx4_args a = id_args(w, x, v, y);
     if (v.pairs > 64 * v.n_expert) return mx4_product_tile(a, ytype, st);
-    return product_mv<true>(a, v.pairs, ytype, st);
+    return product_mv<true>(a, v.pairs / v.n_expert, ytype, st);
+}
+
+// few enough rows that every workgroup may quantise those of its tile
+static bool float_rows(const mx4_args & a, int64_t most) { return a.T <= most && mv_lds(a, 1, MV_WAVES) <= MV_LDS; }
+
+bool mx4_takes_floats(const mx4_mat & w, int64_t x_rows, const moe_view * v) {
+    const mx4_mat x = {nullptr, nullptr, x_rows, w.K};
+    return v ? float_rows(id_args(w, x, *v, nullptr), 16) : float_rows(product_args(w, x, nullptr), 2);
+}
+
+hipError_t mx4_product_float(const mx4_mat & w, int xtype, const void * x, int64_t ldx, int64_t x_rows, const moe_view * v,
+                             int ytype, void * y, hipStream_t st) {
+    const mx4_mat xm = {nullptr, nullptr, x_rows, w.K};
+    return with_type(xtype, [&](auto t) {
+        using X = decltype(t);
+        if (v) return run_mv<1, X, true>(id_args(w, xm, *v, y), (const X *) x, ldx, ytype, st);
+        return run_mv<1, X, false>(product_args(w, xm, y), (const X *) x, ldx, ytype, st);
+    });
 }
 
 }  // namespace mi355x_ops

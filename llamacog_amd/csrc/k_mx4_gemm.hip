@@ -257,13 +257,11 @@ static __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tile(mx4_args a, un
     }
 }
 
-constexpr int64_t MAX_GROUPS = ((int64_t) 1 << 32) / 64 - 1;   // waves of a launch: its threads are counted in 32 bits
-
 template <int FM, int FN, int WM, int WN, bool IDS>
 static hipError_t run_tile(const mx4_args & a, int ytype, hipStream_t st) {
     using S = tile_shape<FM, FN, WM, WN>;
     const int64_t tm = (a.M + S::TM - 1) / S::TM, tn = IDS ? id_tiles(a, S::TN) : (a.T + S::TN - 1) / S::TN;
-    if (tm * tn > MAX_GROUPS / S::NW) return hipErrorInvalidConfiguration;
+    if (tm * tn > MAX_WAVES / S::NW) return hipErrorInvalidConfiguration;
     return with_type(ytype, [&](auto t) {
         using Y = decltype(t);
         auto * k = k_mx4_tile<FM, FN, WM, WN, Y, IDS>;

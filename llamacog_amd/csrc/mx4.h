@@ -109,6 +109,13 @@ struct mx4_args {
 
 hipError_t mx4_product_tile(const mx4_args & a, int ytype, hipStream_t st);   // k_mx4_gemm.hip; by experts with a.offsets
 
+// waves of a launch: its threads are counted in 32 bits
+constexpr int64_t MAX_WAVES = ((int64_t) 1 << 32) / 64 - 1;
+
+// bytes of an x row in shared memory: codes and exponents, an odd number of 16-B columns, so that the
+// same column of 16 rows lies in 16 different ones of the banks
+__host__ __device__ constexpr int mv_row_bytes(int KB) { return (KB + (KB + 15) / 16 | 1) * 16; }
+
 // ---- tiles of sorted pairs -------------------------------------------------------------------
 struct tile_rows {
     int64_t expert;   // -1: rows behind the last expert's
