@@ -142,7 +142,7 @@ double mi355x_bench_op(int which, int64_t a, int64_t b, int iters);
 #define MI355X_MX4 (-4)             // an operand given as MXFP4 codes and scales
 #define MI355X_ERR_TYPE (-1)
 #define MI355X_ERR_SHAPE (-2)
-#define MI355X_ERR_ALIGN (-3)       // codes, y and workspaces 16 bytes, scales 8, the rest its element
+#define MI355X_ERR_ALIGN (-3)       // codes and workspaces 16 bytes, scales 8, the rest its element
 #define MI355X_ERR_WORKSPACE (-4)
 #define MI355X_ERR_HIP (-5)
 

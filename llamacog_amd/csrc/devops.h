@@ -67,8 +67,25 @@ hipError_t moe_combine_back(int type, const void * dy, int64_t lddy, const void 
 template <class T> __device__ __forceinline__ float to_f32(T v) { return (float) v; }
 template <class T> __device__ __forceinline__ T from_f32(float v) { return (T) v; }   // to nearest, ties to even
 
-// N elements moved as one access (N * sizeof(T) <= 16 and a power of two) and widened to float
-template <class T, int N> struct alignas(sizeof(T) * N) pack { T v[N]; };
+// N elements.  16 bytes of them are moved by get and put as one access, at any address that the
+// element allows: gfx950's memory instructions need no more, so rows may lie anywhere.
+template <class T, int N> struct pack { T v[N]; };
+typedef int words16 __attribute__((ext_vector_type(4), aligned(2)));
+
+template <class T, int N> __device__ __forceinline__ pack<T, N> get(const T * p) {
+    static_assert(sizeof(T) * N == 16);
+    const words16 w = *(const words16 *) p;
+    return __builtin_bit_cast(pack<T, N>, w);
+}
+
+// STREAM: past the caches' replacement order, for outputs larger than the Infinity Cache
+constexpr int64_t STREAM_BYTES = (int64_t) 256 << 20;
+template <bool STREAM, class T, int N> __device__ __forceinline__ void put(T * p, const pack<T, N> & v) {
+    static_assert(sizeof(T) * N == 16);
+    const words16 w = __builtin_bit_cast(words16, v);
+    if constexpr (STREAM) __builtin_nontemporal_store(w, (words16 *) p);
+    else *(words16 *) p = w;
+}
 
 // a type as a template argument out of a run-time number: f(T{}) with T = float, _Float16 or __bf16
 template <class F> static inline hipError_t with_type(int type, F && f) {

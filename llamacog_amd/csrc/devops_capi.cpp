@@ -58,12 +58,6 @@ int check_elems(int type, const void * p) {
     return aligned(p, (uintptr_t) elem_size(type)) ? 0 : MI355X_ERR_ALIGN;
 }
 
-// y rows are stored up to 16 bytes at a time where M allows it, which asks for a base to match
-int check_out(int type, const void * p) {
-    if (!is_elem(type)) return MI355X_ERR_TYPE;
-    return aligned(p, 16) ? 0 : MI355X_ERR_ALIGN;
-}
-
 int check_routing(int64_t T, int64_t used) {
     if (T < 0 || used <= 0 || used > MOE_MAX_USED || T * used >= MAX_ROWS) return MI355X_ERR_SHAPE;
     return 0;
@@ -97,7 +91,7 @@ OPS_API int mi355x_mx4_quantize(int xtype, const void * x, int64_t ldx, int64_t 
 OPS_API int mi355x_mx4_dequantize(const uint8_t * codes, const uint8_t * scales, int64_t rows, int64_t K, int ytype, void * y,
                                   void * stream) {
     TRY(check_rows(rows, K));
-    TRY(check_out(ytype, y));
+    TRY(check_elems(ytype, y));
     TRY(check_mx4(codes, scales));
     if (rows == 0) return 0;
     call_stream cs(stream);
@@ -137,7 +131,7 @@ OPS_API int mi355x_mx4_mul_mat(const uint8_t * w_codes, const uint8_t * w_scales
     TRY(check_rows(M, K));
     TRY(check_mx4(w_codes, w_scales));
     TRY(check_x(xtype, x, x_scales, ldx, T, K, work, work_bytes));
-    TRY(check_out(ytype, y));
+    TRY(check_elems(ytype, y));
     if (T == 0 || M == 0) return 0;
     call_stream cs(stream);
     if (cs.err != hipSuccess) return MI355X_ERR_HIP;
@@ -159,7 +153,7 @@ OPS_API int mi355x_mx4_mul_mat_id(const uint8_t * w_codes, const uint8_t * w_sca
     if (n_expert <= 0 || n_expert > MOE_MAX_EXPERTS) return MI355X_ERR_SHAPE;
     const int64_t rows = x_sorted ? T * used : T;
     TRY(check_x(xtype, x, x_scales, ldx, rows, K, work, work_bytes));
-    TRY(check_out(ytype, y));
+    TRY(check_elems(ytype, y));
     if (T == 0 || M == 0) return 0;
     call_stream cs(stream);
     if (cs.err != hipSuccess) return MI355X_ERR_HIP;

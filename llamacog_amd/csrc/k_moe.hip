@@ -20,25 +20,21 @@ static inline unsigned ceil_div(int64_t a, int64_t b) { return (unsigned) ((a + 
 // chunk of pairs, each of its waves one run of it, 64 pairs at a time: lanes with the same expert
 // find each other by one ballot per bit of the id, the lowest of them keeps the wave's count.
 // One chunk is one launch; more are two: the chunks' counts, then their places, where every
-// workgroup sums the counts in front of its own (at most SORT_CHUNKS of them).
+// workgroup sums the counts in front of its own (at most SORT_CHUNKS of them).  Bound by latency:
+// ids are loaded SORT_LOADS at a time, the chunks' counts are summed by all threads.
 constexpr int SORT_WAVES = 16;
-constexpr int SORT_CHUNK = 4096;    // least pairs of a chunk
+constexpr int SORT_LOADS = 4;
+constexpr int SORT_CHUNK = SORT_WAVES * SORT_LOADS * 64;    // least pairs of a chunk
 constexpr int SORT_CHUNKS = 128;
 
-static int64_t sort_chunk(int64_t pairs) {   // pairs per chunk, a multiple of 64 per wave
+static int64_t sort_chunk(int64_t pairs) {   // pairs per chunk
     int64_t c = SORT_CHUNK;
     while ((pairs + c - 1) / c > SORT_CHUNKS) c *= 2;
     return c;
 }
 
-template <class I> __device__ __forceinline__ int expert_of(const I * ids, int64_t p, int64_t end, int n_expert) {
-    if (p >= end) return -1;
-    const I v = ids[p];
-    return v >= 0 && v < (I) n_expert ? (int) v : -1;
-}
-
 // the lanes of the wave whose id is this lane's
-__device__ __forceinline__ unsigned long long same_lanes(int id, int bits) {
+static __device__ __forceinline__ unsigned long long same_lanes(int id, int bits) {
     unsigned long long m = ~0ull;
     for (int b = 0; b < bits; ++b) {
         const unsigned long long set = __ballot((id >> b) & 1);
@@ -47,18 +43,25 @@ __device__ __forceinline__ unsigned long long same_lanes(int id, int bits) {
     return m & __ballot(id >= 0);
 }
 
-template <class I>
-__device__ __forceinline__ void count_run(const I * ids, int64_t p0, int64_t p1, int n_expert, int bits, int * cnt) {
+// f(pair of this lane, its expert or -1, the lanes with the same one) for a wave's run of pairs
+template <class I, class F>
+static __device__ __forceinline__ void for_run(const I * ids, int64_t p0, int64_t p1, int n_expert, int bits, F && f) {
     const int lane = threadIdx.x & 63;
-    for (int64_t p = p0; p < p1; p += 64) {
-        const int id = expert_of(ids, p + lane, p1, n_expert);
-        const unsigned long long m = same_lanes(id, bits);
-        if (id >= 0 && __builtin_ctzll(m) == lane) cnt[id] += __popcll(m);
+    for (int64_t p = p0; p < p1; p += 64 * SORT_LOADS) {
+        I v[SORT_LOADS];
+#pragma unroll
+        for (int i = 0; i < SORT_LOADS; ++i) v[i] = p + 64 * i + lane < p1 ? ids[p + 64 * i + lane] : (I) -1;
+#pragma unroll
+        for (int i = 0; i < SORT_LOADS; ++i) {
+            if (p + 64 * i >= p1) break;
+            const int id = v[i] >= 0 && v[i] < (I) n_expert ? (int) v[i] : -1;
+            f(p + 64 * i + lane, id, same_lanes(id, bits));
+        }
     }
 }
 
 // exclusive prefix over the workgroup's 1024 threads; `total` gets the sum
-__device__ __forceinline__ int block_prefix(int v, int * part, int & total) {
+static __device__ __forceinline__ int block_prefix(int v, int * part, int & total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int upto = v;
 #pragma unroll
@@ -81,20 +84,22 @@ __device__ __forceinline__ int block_prefix(int v, int * part, int & total) {
 
 template <class I, bool COUNT_ONLY>
 static __global__ void __launch_bounds__(64 * SORT_WAVES) k_moe_sort(const I * __restrict__ ids, int64_t pairs, int64_t chunk,
-                                                              int n_expert, int bits, int32_t * __restrict__ counts,
-                                                              int32_t * __restrict__ order, int32_t * __restrict__ rank,
-                                                              int32_t * __restrict__ offsets) {
+                                                                     int n_expert, int bits, int32_t * __restrict__ counts,
+                                                                     int32_t * __restrict__ order, int32_t * __restrict__ rank,
+                                                                     int32_t * __restrict__ offsets) {
     extern __shared__ int cnt[];   // [SORT_WAVES][n_expert]
-    __shared__ int part[SORT_WAVES];
+    __shared__ int part[SORT_WAVES], sums[2][64 * SORT_WAVES];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, e = threadIdx.x;
     const int64_t c0 = (int64_t) blockIdx.x * chunk, c1 = min(c0 + chunk, pairs);
     const int64_t run = chunk / SORT_WAVES;
     const int64_t p0 = min(c0 + wave * run, c1), p1 = min(p0 + run, c1);
-    for (int i = threadIdx.x; i < SORT_WAVES * n_expert; i += 64 * SORT_WAVES) cnt[i] = 0;
-    __syncthreads();
-    count_run(ids, p0, p1, n_expert, bits, cnt + wave * n_expert);
-    __syncthreads();
+    int * mine = cnt + wave * n_expert;
+    for (int i = lane; i < n_expert; i += 64) mine[i] = 0;
+    for_run(ids, p0, p1, n_expert, bits, [&](int64_t, int id, unsigned long long m) {
+        if (id >= 0 && __builtin_ctzll(m) == lane) mine[id] += __popcll(m);
+    });
     if (COUNT_ONLY) {
+        __syncthreads();
         if (e < n_expert) {
             int s = 0;
 #pragma unroll
@@ -103,17 +108,32 @@ static __global__ void __launch_bounds__(64 * SORT_WAVES) k_moe_sort(const I * _
         }
         return;
     }
-    // expert e's pairs in all chunks, and in those before this one
+    // expert e's pairs in all chunks, and in those before this one: `share` threads for each expert
+    if (gridDim.x > 1) {
+        const int share = 64 * SORT_WAVES / n_expert;
+        const int ex = threadIdx.x % n_expert, first = threadIdx.x / n_expert;
+        int all = 0, before = 0;
+        if (first < share) {
+#pragma unroll 8
+            for (int c = first; c < (int) gridDim.x; c += share) {
+                const int s = counts[(int64_t) c * n_expert + ex];
+                before += c < (int) blockIdx.x ? s : 0;
+                all += s;
+            }
+        }
+        sums[0][threadIdx.x] = all;
+        sums[1][threadIdx.x] = before;
+    }
+    __syncthreads();
     int all = 0, before = 0;
     if (e < n_expert) {
         if (gridDim.x == 1) {
 #pragma unroll
             for (int w = 0; w < SORT_WAVES; ++w) all += cnt[w * n_expert + e];
         } else {
-            for (int c = 0; c < (int) gridDim.x; ++c) {
-                const int s = counts[(int64_t) c * n_expert + e];
-                before += c < (int) blockIdx.x ? s : 0;
-                all += s;
+            for (int k = 0; k < 64 * SORT_WAVES / n_expert; ++k) {
+                all += sums[0][k * n_expert + e];
+                before += sums[1][k * n_expert + e];
             }
         }
     }
@@ -131,22 +151,19 @@ static __global__ void __launch_bounds__(64 * SORT_WAVES) k_moe_sort(const I * _
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) offsets[n_expert] = held;
     __syncthreads();
-    int * mine = cnt + wave * n_expert;
-    for (int64_t p = p0; p < p1; p += 64) {
-        const int id = expert_of(ids, p + lane, p1, n_expert);
-        const unsigned long long m = same_lanes(id, bits);
+    for_run(ids, p0, p1, n_expert, bits, [&](int64_t p, int id, unsigned long long m) {
         int place = -1;
         if (id >= 0) {
             place = mine[id] + __popcll(m & ((1ull << lane) - 1));
-            order[place] = (int32_t) (p + lane);
+            order[place] = (int32_t) p;
         }
-        if (p + lane < p1) {
-            rank[p + lane] = place;
-            if (p + lane >= held) order[p + lane] = -1;
+        if (p < p1) {
+            rank[p] = place;
+            if (p >= held) order[p] = -1;
         }
         // the places above are read before the count moves on: one wave, in order
         if (id >= 0 && __builtin_ctzll(m) == lane) mine[id] += __popcll(m);
-    }
+    });
 }
 
 size_t moe_sort_workspace(int64_t pairs, int n_expert) {
@@ -175,145 +192,163 @@ hipError_t moe_sort(const void * ids, int id_bytes, int64_t pairs, int n_expert,
 
 // ---- rows ------------------------------------------------------------------------------------
 // All three are bound by memory: every row is read once and written once, a token's row once for
-// all of its slots (the gather goes by rank, not by order, for that).  A lane owns N columns of a
-// token; lanes are laid over the columns in a power of two.
+// all of its slots (the gather goes by rank, not by order, for that).  A lane owns 16 bytes of a
+// token's columns, the last one what is left; lanes are laid over the columns in a power of two.
+// Rows lie on any address.
 struct row_args {
     int64_t T, D, pairs;
     int used, lsh;   // slots; log2 of the lanes over a row
 };
 
-__device__ __forceinline__ bool my_columns(const row_args & a, int N, int64_t & t, int64_t & col) {
+template <class T> constexpr int COLS = 16 / sizeof(T);
+
+static __device__ __forceinline__ bool my_columns(const row_args & a, int N, int64_t & t, int64_t & col) {
     col = ((int64_t) blockIdx.y << a.lsh | (threadIdx.x & ((1 << a.lsh) - 1))) * N;
     t = (int64_t) blockIdx.x * (256 >> a.lsh) + (threadIdx.x >> a.lsh);
     return t < a.T && col < a.D;
 }
 
-template <class T, int N>
+// n elements of a row from `p` on, in one access if it is all N, zeros behind them; WHOLE: it always is
+template <bool WHOLE, class T, int N> static __device__ __forceinline__ pack<T, N> take(const T * p, int64_t n) {
+    if (WHOLE || n >= N) return get<T, N>(p);
+    pack<T, N> v = {};
+    for (int i = 0; i < N; ++i)
+        if (i < n) v.v[i] = p[i];
+    return v;
+}
+template <bool WHOLE, bool STREAM, class T, int N> static __device__ __forceinline__ void give(T * p, int64_t n, const pack<T, N> & v) {
+    if (WHOLE || n >= N) return put<STREAM>(p, v);
+    for (int i = 0; i < N; ++i)
+        if (i < n) p[i] = v.v[i];
+}
+
+template <class T, bool WHOLE, bool STREAM>
 static __global__ void __launch_bounds__(256) k_moe_gather(row_args a, const T * __restrict__ x, int64_t ldx,
-                                                    const int32_t * __restrict__ order, const int32_t * __restrict__ rank,
-                                                    T * __restrict__ xs) {
-    using V = pack<T, N>;
+                                                           const int32_t * __restrict__ order,
+                                                           const int32_t * __restrict__ rank, T * __restrict__ xs) {
     int64_t t, col;
-    if (!my_columns(a, N, t, col)) return;
-    const V v = *(const V *) (x + t * ldx + col);
+    if (!my_columns(a, COLS<T>, t, col)) return;
+    const int64_t n = a.D - col;
+    const pack<T, COLS<T>> v = take<WHOLE, T, COLS<T>>(x + t * ldx + col, n);
     for (int j = 0; j < a.used; ++j) {
         const int64_t p = t * a.used + j, r = rank[p];
-        if (r >= 0 && r < a.pairs) *(V *) (xs + r * a.D + col) = v;
-        if (order[p] < 0) *(V *) (xs + p * a.D + col) = V{};
+        if (r >= 0 && r < a.pairs) give<WHOLE, STREAM>(xs + r * a.D + col, n, v);
+        if (order[p] < 0) give<WHOLE, STREAM>(xs + p * a.D + col, n, pack<T, COLS<T>>{});
     }
 }
 
-template <class T, int N, bool WEIGHTED>
+template <class T, bool WHOLE, bool WEIGHTED>
 static __global__ void __launch_bounds__(256) k_moe_combine(row_args a, const T * __restrict__ ys, int64_t ldys,
-                                                     const int32_t * __restrict__ rank, const float * __restrict__ w,
-                                                     T * __restrict__ y) {
-    using V = pack<T, N>;
+                                                            const int32_t * __restrict__ rank, const float * __restrict__ w,
+                                                            T * __restrict__ y) {
+    constexpr int N = COLS<T>;
     int64_t t, col;
     if (!my_columns(a, N, t, col)) return;
     float s[N] = {};
-    for (int j = 0; j < a.used; ++j) {
-        const int64_t p = t * a.used + j, r = rank[p];
-        if (r < 0 || r >= a.pairs) continue;   // whatever the weight and the row behind it hold
-        const V v = *(const V *) (ys + r * ldys + col);
-        const float f = WEIGHTED ? w[p] : 1.0f;
+    constexpr int BATCH = 4;   // rows on their way at a time
+    for (int j0 = 0; j0 < a.used; j0 += BATCH) {
+        pack<T, N> v[BATCH];
+        float f[BATCH];
 #pragma unroll
-        for (int i = 0; i < N; ++i) s[i] = fmaf(f, to_f32(v.v[i]), s[i]);
+        for (int k = 0; k < BATCH; ++k) {
+            const int64_t p = t * a.used + j0 + k, r = j0 + k < a.used ? rank[p] : -1;
+            // a slot without an expert adds zero, whatever the weight and the row behind it hold
+            const bool held = r >= 0 && r < a.pairs;
+            v[k] = held ? take<WHOLE, T, N>(ys + r * ldys + col, a.D - col) : pack<T, N>{};
+            f[k] = !held ? 0.0f : WEIGHTED ? w[p] : 1.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k)
+#pragma unroll
+            for (int i = 0; i < N; ++i) s[i] = fmaf(f[k], to_f32(v[k].v[i]), s[i]);
     }
-    V o;
+    pack<T, N> o;
 #pragma unroll
     for (int i = 0; i < N; ++i) o.v[i] = from_f32<T>(s[i]);
-    *(V *) (y + t * a.D + col) = o;
+    give<WHOLE, false>(y + t * a.D + col, a.D - col, o);
 }
 
-// one workgroup per token: its dy row once, each slot's row read and its gradient written, the dot
-// products joined in shared memory in a fixed order.  A lane's columns are 16 bytes wide whatever the
-// access width A, so that the sums do not depend on alignment.
-template <class T, int A>
+// Each slot's row read and its gradient written; a token's lanes (up to a workgroup) go through its
+// columns and join their dot products, in a wave by exchanges, over waves in shared memory, always
+// in the same order.
+template <class T, bool WHOLE, bool STREAM>
 static __global__ void __launch_bounds__(256) k_moe_combine_back(row_args a, const T * __restrict__ dy, int64_t lddy,
                                                                  const T * __restrict__ ys, int64_t ldys,
                                                                  const int32_t * __restrict__ order,
                                                                  const int32_t * __restrict__ rank,
                                                                  const float * __restrict__ w, T * __restrict__ dys,
                                                                  float * __restrict__ dw) {
-    using V = pack<T, A>;
-    constexpr int N = 16 / sizeof(T);
-    __shared__ float part[MOE_MAX_USED][4];
-    const int64_t t = blockIdx.x;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int N = COLS<T>;
+    __shared__ float part[4][MOE_MAX_USED];
+    const int lanes = 1 << a.lsh, mine = threadIdx.x & (lanes - 1);
+    const int64_t t = (int64_t) blockIdx.x * (256 >> a.lsh) + (threadIdx.x >> a.lsh);
+    const bool here = t < a.T;
     for (int j = 0; j < a.used; ++j) {
-        const int64_t p = t * a.used + j, r = rank[p];
-        const bool held = r >= 0 && r < a.pairs, empty = order[p] < 0;
-        const float f = w[p];
         float dot = 0.0f;
-        for (int64_t col = (int64_t) threadIdx.x * N; col < a.D; col += 256 * N) {
-#pragma unroll
-            for (int i = 0; i < N; i += A) {
-                if (col + i >= a.D) break;   // D is a multiple of A
+        if (here) {
+            const int64_t p = t * a.used + j, r = rank[p];
+            const bool held = r >= 0 && r < a.pairs, empty = order[p] < 0;
+            const float f = w[p];
+            for (int64_t col = (int64_t) mine * N; col < a.D; col += lanes * N) {
+                const int64_t n = a.D - col;
                 if (held) {
-                    const V g = *(const V *) (dy + t * lddy + col + i), v = *(const V *) (ys + r * ldys + col + i);
-                    V o;
+                    const pack<T, N> g = take<WHOLE, T, N>(dy + t * lddy + col, n), v = take<WHOLE, T, N>(ys + r * ldys + col, n);
+                    pack<T, N> o;
 #pragma unroll
-                    for (int k = 0; k < A; ++k) {
-                        dot = fmaf(to_f32(g.v[k]), to_f32(v.v[k]), dot);
-                        o.v[k] = from_f32<T>(f * to_f32(g.v[k]));
+                    for (int i = 0; i < N; ++i) {
+                        dot = fmaf(to_f32(g.v[i]), to_f32(v.v[i]), dot);
+                        o.v[i] = from_f32<T>(f * to_f32(g.v[i]));
                     }
-                    *(V *) (dys + r * a.D + col + i) = o;
+                    give<WHOLE, STREAM>(dys + r * a.D + col, n, o);
                 }
-                if (empty) *(V *) (dys + p * a.D + col + i) = V{};
+                if (empty) give<WHOLE, STREAM>(dys + p * a.D + col, n, pack<T, N>{});
             }
         }
-#pragma unroll
-        for (int d = 32; d; d >>= 1) dot += __shfl_xor(dot, d);
-        if (lane == 0) part[j][wave] = held ? dot : 0.0f;
+        for (int d = min(lanes, 64) / 2; d; d >>= 1) dot += __shfl_xor(dot, d);
+        if (lanes <= 64) {
+            if (here && mine == 0) dw[t * a.used + j] = dot;
+        } else if ((threadIdx.x & 63) == 0) {
+            part[threadIdx.x >> 6][j] = dot;
+        }
     }
+    if (lanes <= 64) return;
     __syncthreads();
-    if ((int) threadIdx.x < a.used) {
-        const float * q = part[threadIdx.x];
-        dw[t * a.used + threadIdx.x] = (q[0] + q[1]) + (q[2] + q[3]);
+    if (here && mine < a.used) {
+        const int wave = threadIdx.x >> 6;
+        float s = part[wave][mine] + part[wave + 1][mine];
+        if (lanes == 256) s += part[2][mine] + part[3][mine];
+        dw[t * a.used + mine] = s;
     }
 }
 
-// the widest access that every row and base allows: f(type, columns per lane)
-template <class F> static hipError_t with_columns(int type, int64_t D, uintptr_t bases, int64_t lds, F && f) {
+// f(element type, WHOLE, a flag) as template arguments, the layout of the rows and the groups of tokens and columns
+template <class F> static hipError_t with_rows(int type, int64_t T, int64_t D, int used, bool flag, F && f) {
     return with_type(type, [&](auto t) {
-        using T = decltype(t);
-        constexpr int W = 16 / sizeof(T);
-        const int64_t step = D | lds;
-        auto fits = [&](int n) { return step % n == 0 && bases % (n * sizeof(T)) == 0; };
-        if (fits(W)) return f(t, std::integral_constant<int, W>{});
-        if (fits(W / 2)) return f(t, std::integral_constant<int, W / 2>{});
-        if (W > 4 && fits(2)) return f(t, std::integral_constant<int, 2>{});
-        return f(t, std::integral_constant<int, 1>{});
+        using E = decltype(t);
+        row_args a{T, D, T * used, used, 0};
+        const int64_t cols = (D + COLS<E> - 1) / COLS<E>;
+        while (a.lsh < 8 && (1 << a.lsh) < cols) ++a.lsh;
+        const dim3 grid(ceil_div(T, 256 >> a.lsh), ceil_div(cols, (int64_t) 1 << a.lsh));
+        auto with_flag = [&](auto whole) { return flag ? f(t, whole, std::true_type{}, a, grid) : f(t, whole, std::false_type{}, a, grid); };
+        return D % COLS<E> == 0 ? with_flag(std::true_type{}) : with_flag(std::false_type{});
     });
-}
-
-static row_args row_layout(int64_t T, int64_t D, int used, int N, dim3 & grid) {
-    row_args a{T, D, T * used, used, 0};
-    const int64_t cols = (D + N - 1) / N;
-    while (a.lsh < 8 && (1 << a.lsh) < cols) ++a.lsh;
-    grid = dim3(ceil_div(T, 256 >> a.lsh), ceil_div(cols, (int64_t) 1 << a.lsh));
-    return a;
 }
 
 hipError_t moe_gather(int type, const void * x, int64_t ldx, int64_t T, int64_t D, int used, const int32_t * order,
                       const int32_t * rank, void * xs, hipStream_t st) {
-    return with_columns(type, D, (uintptr_t) x | (uintptr_t) xs, ldx, [&](auto t, auto n) {
+    const bool stream = T * used * D * (type == ELEM_F32 ? 4 : 2) > STREAM_BYTES;
+    return with_rows(type, T, D, used, stream, [&](auto t, auto whole, auto flag, const row_args & a, dim3 grid) {
         using E = decltype(t);
-        dim3 grid;
-        const row_args a = row_layout(T, D, used, n, grid);
-        k_moe_gather<E, n><<<grid, 256, 0, st>>>(a, (const E *) x, ldx, order, rank, (E *) xs);
+        k_moe_gather<E, whole, flag><<<grid, 256, 0, st>>>(a, (const E *) x, ldx, order, rank, (E *) xs);
         return hipGetLastError();
     });
 }
 
 hipError_t moe_combine(int type, const void * ys, int64_t ldys, int64_t T, int64_t D, int used, const int32_t * rank,
                        const float * w, void * y, hipStream_t st) {
-    return with_columns(type, D, (uintptr_t) ys | (uintptr_t) y, ldys, [&](auto t, auto n) {
+    return with_rows(type, T, D, used, w != nullptr, [&](auto t, auto whole, auto flag, const row_args & a, dim3 grid) {
         using E = decltype(t);
-        dim3 grid;
-        const row_args a = row_layout(T, D, used, n, grid);
-        if (w) k_moe_combine<E, n, true><<<grid, 256, 0, st>>>(a, (const E *) ys, ldys, rank, w, (E *) y);
-        else k_moe_combine<E, n, false><<<grid, 256, 0, st>>>(a, (const E *) ys, ldys, rank, w, (E *) y);
+        k_moe_combine<E, whole, flag><<<grid, 256, 0, st>>>(a, (const E *) ys, ldys, rank, w, (E *) y);
         return hipGetLastError();
     });
 }
@@ -321,11 +356,11 @@ hipError_t moe_combine(int type, const void * ys, int64_t ldys, int64_t T, int64
 hipError_t moe_combine_back(int type, const void * dy, int64_t lddy, const void * ys, int64_t ldys, int64_t T, int64_t D,
                             int used, const int32_t * order, const int32_t * rank, const float * w, void * dys, float * dw,
                             hipStream_t st) {
-    return with_columns(type, D, (uintptr_t) dy | (uintptr_t) ys | (uintptr_t) dys, lddy | ldys, [&](auto t, auto n) {
+    const bool stream = T * used * D * (type == ELEM_F32 ? 4 : 2) > STREAM_BYTES;
+    return with_rows(type, T, D, used, stream, [&](auto t, auto whole, auto flag, const row_args & a, dim3 grid) {
         using E = decltype(t);
-        const row_args a{T, D, T * used, used, 0};
-        k_moe_combine_back<E, n><<<(unsigned) T, 256, 0, st>>>(a, (const E *) dy, lddy, (const E *) ys, ldys, order, rank, w,
-                                                                (E *) dys, dw);
+        k_moe_combine_back<E, whole, flag><<<grid.x, 256, 0, st>>>(a, (const E *) dy, lddy, (const E *) ys, ldys, order, rank, w,
+                                                                   (E *) dys, dw);
         return hipGetLastError();
     });
 }

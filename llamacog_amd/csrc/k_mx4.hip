@@ -20,7 +20,7 @@ static inline unsigned ceil_div(int64_t a, int64_t b) { return (unsigned) ((a + 
 // times as many rows as its lanes hold, loads first, to keep bytes in flight.
 constexpr int QROWS = 4;
 
-template <class T, bool VEC>
+template <class T>
 static __global__ void __launch_bounds__(256) k_mx4_quantize(const T * __restrict__ x, int64_t ldx, int64_t rows, int64_t K, int lsh,
                                                       uint8_t * __restrict__ codes, uint8_t * __restrict__ scales) {
     const int64_t c = (int64_t) blockIdx.y << lsh | (threadIdx.x & ((1 << lsh) - 1));
@@ -31,7 +31,7 @@ static __global__ void __launch_bounds__(256) k_mx4_quantize(const T * __restric
 #pragma unroll
     for (int i = 0; i < QROWS; ++i) {
         const int64_t row = min(row0 + (int64_t) i * rp, rows - 1);
-        load8<T, VEC>(x + row * ldx + c * 8, v[i]);
+        load8(x + row * ldx + c * 8, v[i]);
     }
 #pragma unroll
     for (int i = 0; i < QROWS; ++i) {
@@ -61,10 +61,7 @@ hipError_t mx4_quantize(int type, const void * x, int64_t ldx, int64_t rows, int
     const dim3 grid(ceil_div(rows, (int64_t) (256 >> lsh) * QROWS), ceil_div(K / 8, 1 << lsh));
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        // a lane's 8 elements are read with 16-B accesses where every row starts on 16 B
-        const bool vec = ((uintptr_t) x % 16 == 0) && (ldx * (int64_t) sizeof(T) % 16 == 0);
-        if (vec) k_mx4_quantize<T, true><<<grid, 256, 0, st>>>((const T *) x, ldx, rows, K, lsh, codes, scales);
-        else k_mx4_quantize<T, false><<<grid, 256, 0, st>>>((const T *) x, ldx, rows, K, lsh, codes, scales);
+        k_mx4_quantize<T><<<grid, 256, 0, st>>>((const T *) x, ldx, rows, K, lsh, codes, scales);
         return hipGetLastError();
     });
 }
@@ -176,13 +173,11 @@ static __global__ void __launch_bounds__(64 * MV_WAVES, 4) k_mx4_mv(mx4_args a, 
             }
         }
     } else {
-        const bool vec = (uintptr_t) x % 16 == 0 && ldx * (int64_t) sizeof(X) % 16 == 0;
         for (int t = 0; t < tr.n; ++t) {
             const X * row = x + x_row<IDS>(a, tr.first + t) * ldx;
             for (int c = threadIdx.x; c < a.KB * 4; c += 64 * MV_WAVES) {
                 float v[8];
-                if (vec) load8<X, true>(row + (int64_t) c * 8, v);
-                else load8<X, false>(row + (int64_t) c * 8, v);
+                load8(row + (int64_t) c * 8, v);
                 const unsigned e = mx4_block_exponent(v);
                 *(uint32_t *) (lds + t * row_bytes + c * 4) = mx4_pack8(v, e);
                 if ((c & 3) == 0) lds[t * row_bytes + a.KB * 16 + (c >> 2)] = (uint8_t) e;

@@ -211,7 +211,6 @@ static __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tile(mx4_args a, un
     constexpr int PASSES = (S::TN * ROW + S::LDS - 1) / S::LDS, PT = S::TN / PASSES;
     static_assert(PT % 32 == 0 && PT * ROW <= S::LDS, "whole fragments in a pass");
     const int cols = (int) min((int64_t) S::TM, a.M - m0);
-    const bool wide = a.M * (int64_t) sizeof(Y) % 16 == 0;
     Y * out = y + tr.first * a.M + m0;
 #pragma unroll
     for (int pass = 0; pass < PASSES; ++pass) {
@@ -227,22 +226,23 @@ static __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tile(mx4_args a, un
                     pack<Y, 4> q;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) q.v[k] = from_f32<Y>(acc[m][n][i + k]);
-                    *(pack<Y, 4> *) (lds + (t + r31) * ROW + (wm + m * 32 + 2 * i + 4 * half) * sizeof(Y)) = q;
+                    char * to = lds + (t + r31) * ROW + (wm + m * 32 + 2 * i + 4 * half) * (int) sizeof(Y);
+                    __builtin_memcpy(__builtin_assume_aligned(to, sizeof(q)), &q, sizeof(q));
                 }
         }
         __syncthreads();
         const int rows = (int) min((int64_t) PT, tr.n - pass * PT);
-        if (wide) {
-            constexpr int V = 16 / sizeof(Y), PER = S::TM / V;
-            for (int i = threadIdx.x; i < rows * PER; i += 64 * S::NW)
-                if (i % PER * V < cols)
-                    *(pack<Y, V> *) (out + (int64_t) (pass * PT + i / PER) * a.M + i % PER * V) =
-                        *(const pack<Y, V> *) (lds + i / PER * ROW + i % PER * 16);
-        } else {
-            for (int i = threadIdx.x; i < rows * S::TM; i += 64 * S::NW)
-                if (i % S::TM < cols)
-                    out[(int64_t) (pass * PT + i / S::TM) * a.M + i % S::TM] =
-                        *(const Y *) (lds + i / S::TM * ROW + i % S::TM * (int) sizeof(Y));
+        constexpr int V = 16 / sizeof(Y), PER = S::TM / V;
+        for (int i = threadIdx.x; i < rows * PER; i += 64 * S::NW) {
+            const int c = i % PER * V;
+            if (c >= cols) continue;
+            pack<Y, V> q;
+            __builtin_memcpy(&q, __builtin_assume_aligned(lds + i / PER * ROW + i % PER * 16, 16), 16);
+            Y * to = out + (int64_t) (pass * PT + i / PER) * a.M + c;
+            if (c + V <= cols) put<false>(to, q);
+            else
+                for (int k = 0; k < V; ++k)
+                    if (c + k < cols) to[k] = q.v[k];
         }
     }
 }

@@ -11,18 +11,13 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 
 // ---- elements --------------------------------------------------------------------------------
-template <class T, bool VEC> __device__ __forceinline__ void load8(const T * p, float (&v)[8]) {
-    if constexpr (VEC) {
-        constexpr int N = 16 / sizeof(T);
+template <class T> __device__ __forceinline__ void load8(const T * p, float (&v)[8]) {
+    constexpr int N = 16 / sizeof(T);
 #pragma unroll
-        for (int i = 0; i < 8; i += N) {
-            const pack<T, N> q = *(const pack<T, N> *) (p + i);
+    for (int i = 0; i < 8; i += N) {
+        const pack<T, N> q = get<T, N>(p + i);
 #pragma unroll
-            for (int j = 0; j < N; ++j) v[i + j] = to_f32(q.v[j]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_f32(p[i]);
+        for (int j = 0; j < N; ++j) v[i + j] = to_f32(q.v[j]);
     }
 }
 
@@ -33,7 +28,7 @@ template <class T> __device__ __forceinline__ void store8(T * p, const float (&v
         pack<T, N> q;
 #pragma unroll
         for (int j = 0; j < N; ++j) q.v[j] = from_f32<T>(v[i + j]);
-        *(pack<T, N> *) (p + i) = q;
+        put<false>(p + i, q);
     }
 }
 

@@ -176,7 +176,7 @@ REFUSED = [
     ("mi355x_mx4_quantize", (1, A, 64, 3, 64, A, A + 4), -3),
     ("mi355x_mx4_dequantize", (A, A, 3, 64, 39, A), -1),
     ("mi355x_mx4_dequantize", (A, A, 3, 40, 0, A), -2),
-    ("mi355x_mx4_dequantize", (A, A, 3, 64, 0, A + 4), -3),
+    ("mi355x_mx4_dequantize", (A, A, 3, 64, 0, A + 2), -3),
     ("mi355x_mx4_mul_mat", (A, A, 8, 64, 12, A, None, 64, 3, 0, A, A, 1 << 20), -1),
     ("mi355x_mx4_mul_mat", (A, A, 8, 64, 0, A, None, 64, 3, 8, A, A, 1 << 20), -1),
     ("mi355x_mx4_mul_mat", (A, A, 8, 65, 0, A, None, 64, 3, 0, A, A, 1 << 20), -2),
