@@ -143,7 +143,7 @@ static __global__ void __launch_bounds__(64 * MV_WAVES, 4) k_mx4_mv(mx4_args a, 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, q = lane >> 4, part = wave % KS;
     const int64_t tile = blockIdx.x / per_tile;
-    const tile_rows tr = IDS ? find_tile(a, tile, 16 * NT)
+    const tile_rows tr = IDS ? tile_scan(a, 16 * NT).tile(a, tile)
                              : tile_rows{0, tile * 16 * NT, min((int64_t) 16 * NT, a.T - tile * 16 * NT)};
     if (tr.n <= 0) return;
     Y * y = (Y *) a.y + tr.first * a.M;

@@ -97,9 +97,18 @@ static __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tile(mx4_args a, un
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     unsigned tm, tn;
-    tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+    tile_rows tr;
+    if constexpr (IDS) {
+        const tile_scan scan(a, S::TN);
+        tiles_n = (unsigned) scan.tiles(a);   // the launch is for any routing
+        if (blockIdx.x >= tiles_m * tiles_n) return;
+        tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+        tr = scan.tile(a, tn);
+    } else {
+        tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+        tr = {0, (int64_t) tn * S::TN, min((int64_t) S::TN, a.T - (int64_t) tn * S::TN)};
+    }
     const int64_t m0 = (int64_t) tm * S::TM;
-    const tile_rows tr = IDS ? find_tile(a, tn, S::TN) : tile_rows{0, (int64_t) tn * S::TN, min((int64_t) S::TN, a.T - (int64_t) tn * S::TN)};
     if (tr.n <= 0) return;
     Y * y = (Y *) a.y;
     if (IDS && tr.expert < 0) {   // pairs that no expert takes
@@ -188,6 +197,15 @@ static __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tile(mx4_args a, un
     for (int h = 0; h < STAGES - 1; ++h) unroll<COPIES>([&](auto c) { copy(h, c); });
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(AHEAD) : "memory");
     unroll<INS>([&](auto i) { copies(STAGES - 1, FIRST, i); });
+    // a wave whose part of the tile lies past M or the tile's rows only copies: its results are not
+    // stored, and the others have the matrix cores to themselves
+    if (m0 + wm >= a.M || wn - S::TM >= tr.n) {
+        for (int h = 0; h < last; ++h) {
+            unroll<INS>([&](auto i) { copies(h + STAGES - 1, SECOND, i); });
+            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(AHEAD) : "memory");
+            unroll<INS>([&](auto i) { copies(h + STAGES, FIRST, i); });
+        }
+    } else {
     unroll<FR>([&](auto i) { f0.template load<i>(ca + slot[0], cb + slot[0]); });
     load_exps(0);
     take_exps(0);
@@ -202,6 +220,7 @@ static __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tile(mx4_args a, un
     }
     mma_step<0>(acc, f0, sa, sb, [&](auto i) { reads(f1, at, 1, i); });
     mma_step<1>(acc, f1, sa, sb, [](auto) {});
+    }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no copy is left when the shared memory gets another use
 
     // The results go out through shared memory: straight from the registers a store would touch 32 x

@@ -125,48 +125,60 @@ static inline int64_t id_tiles(const mx4_args & a, int rows) {
     return a.T / rows + used + 1;
 }
 
-// the tile-th tile of `rows` sorted rows, experts in order, the rows that no expert takes last.
-// Every wave finds it by itself: lane l counts the tiles of its ceil(n_expert / 64) experts.
-__device__ __forceinline__ tile_rows find_tile(const mx4_args & a, int64_t tile, int rows) {
-    const int lane = threadIdx.x & 63;
-    const int per = (a.n_expert + 63) / 64;
-    const int e0 = min(lane * per, a.n_expert), e1 = min(e0 + per, a.n_expert);
-    int mine = 0;
-    for (int e = e0; e < e1; ++e) mine += (a.offsets[e + 1] - a.offsets[e] + rows - 1) / rows;
-    int upto = mine;
+// The tiles of `rows` sorted rows: experts in order, then the rows that no expert takes.  Every wave
+// counts them by itself, lane l those of its ceil(n_expert / 64) experts.
+struct tile_scan {
+    int e0, e1, mine, upto;   // this lane's experts and tiles, and the tiles up to them
+    int total, held;          // all experts' tiles, their rows
+    int rows;
+
+    __device__ __forceinline__ tile_scan(const mx4_args & a, int rows) : rows(rows) {
+        const int lane = threadIdx.x & 63;
+        const int per = (a.n_expert + 63) / 64;
+        e0 = min(lane * per, a.n_expert);
+        e1 = min(e0 + per, a.n_expert);
+        mine = 0;
+        for (int e = e0; e < e1; ++e) mine += (a.offsets[e + 1] - a.offsets[e] + rows - 1) / rows;
+        upto = mine;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(upto, d);
-        if (lane >= d) upto += o;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(upto, d);
+            if (lane >= d) upto += o;
+        }
+        total = max(0, __builtin_amdgcn_readlane(upto, 63));
+        held = max(0, __builtin_amdgcn_readfirstlane(a.offsets[a.n_expert]));
     }
-    const int total = __builtin_amdgcn_readlane(upto, 63);
-    const int held = a.offsets[a.n_expert];
-    tile_rows tr;
-    if (tile >= total) {
-        tr.expert = -1;
-        tr.first = max(0, held) + (tile - total) * rows;
-        tr.n = max((int64_t) 0, min((int64_t) rows, a.T - tr.first));
+    // with the rest's
+    __device__ __forceinline__ int64_t tiles(const mx4_args & a) const { return total + max((int64_t) 0, (a.T - held + rows - 1) / rows); }
+
+    __device__ __forceinline__ tile_rows tile(const mx4_args & a, int64_t i) const {
+        tile_rows tr;
+        if (i >= total) {
+            tr.expert = -1;
+            tr.first = held + (i - total) * rows;
+            tr.n = max((int64_t) 0, min((int64_t) rows, a.T - tr.first));
+            return tr;
+        }
+        const unsigned long long hit = __ballot(upto > (int) i);
+        const int owner = (int) __builtin_ctzll(hit);
+        int e = e0, first = 0, n = 0;
+        if ((int) (threadIdx.x & 63) == owner) {
+            int left = (int) i - (upto - mine);
+            for (;; ++e) {
+                n = a.offsets[e + 1] - a.offsets[e];
+                const int t = (n + rows - 1) / rows;
+                if (left < t || e + 1 >= e1) break;
+                left -= t;
+            }
+            first = a.offsets[e] + left * rows;
+            n = min(rows, n - left * rows);
+        }
+        tr.expert = __builtin_amdgcn_readlane(e, owner);
+        tr.first = max(0, __builtin_amdgcn_readlane(first, owner));
+        tr.n = min((int64_t) __builtin_amdgcn_readlane(n, owner), a.T - tr.first);   // whatever the offsets hold
         return tr;
     }
-    const unsigned long long hit = __ballot(upto > (int) tile);
-    const int owner = (int) __builtin_ctzll(hit);
-    int e = e0, first = 0, n = 0;
-    if (lane == owner) {
-        int left = (int) tile - (upto - mine);
-        for (;; ++e) {
-            n = a.offsets[e + 1] - a.offsets[e];
-            const int t = (n + rows - 1) / rows;
-            if (left < t || e + 1 >= e1) break;
-            left -= t;
-        }
-        first = a.offsets[e] + left * rows;
-        n = min(rows, n - left * rows);
-    }
-    tr.expert = __builtin_amdgcn_readlane(e, owner);
-    tr.first = max(0, __builtin_amdgcn_readlane(first, owner));
-    tr.n = min((int64_t) __builtin_amdgcn_readlane(n, owner), a.T - tr.first);   // whatever the offsets hold
-    return tr;
-}
+};
 
 // the x row of y row p, inside the matrix whatever the order holds
 template <bool IDS> __device__ __forceinline__ int64_t x_row(const mx4_args & a, int64_t p) {
