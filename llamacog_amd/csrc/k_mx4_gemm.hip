@@ -1,15 +1,14 @@
 // k_mx4_gemm.hip — the MXFP4 product for many rows, dense and by experts: tiles on
 // v_mfma_scale_f32_32x32x64 (both operands FP4).
 //
-// A workgroup of WM x WN waves computes TM = 32 FM WM weight rows by TN = 32 FN WN x rows, a panel of
-// 128 elements of K at a time.  Both operands' codes (64 B of a row) and exponents (4 B) go from
-// memory to shared memory without registers, into a ring of STAGES panels: copies have most of
-// STAGES - 1 panels' arithmetic to arrive in, more than memory takes under load.
+// A workgroup of WM x WN waves computes TM = 32 FM WM weight rows by TN = 32 FN WN x rows, a plane of
+// 256 elements of K at a time.  Both operands' codes (128 B of a row, a cache line) and exponents
+// (8 B) go from memory to shared memory without registers, into a ring of STAGES planes.
 //   - The 32x32x64 instruction wants from lane l 32 consecutive elements of row l % 32, and their
 //     exponent in a byte of a register that the instruction names.  Which 32-blocks of K meet in an
-//     instruction is free as long as both operands agree: step j of a panel takes block j from lanes
-//     0-31 and block 2 + j from lanes 32-63.
-//   - Row r's 16-B block b lies in slot b ^ (r / 4 % 4): the 64 banks hold four rows, so that any 16
+//     instruction is free as long as both operands agree: step j of a plane takes block j from lanes
+//     0-31 and block 4 + j from lanes 32-63, so that a lane's four exponents are one aligned word.
+//   - Row r's 16-B block b lies in slot b ^ (r / 2 % 8): the 64 banks hold two rows, so that any 16
 //     rows that differ mod 16 are read without a conflict.  The copies to shared memory can only
 //     write lane after lane, so the order is made on the reading side: each lane fetches the block
 //     that belongs in its slot.
@@ -17,6 +16,7 @@
 //   - Past M and T rows repeat the last one; their results are not stored.
 #include "mx4.h"
 
+#include <algorithm>
 #include <cmath>
 #include <utility>
 
@@ -42,10 +42,10 @@ template <int J> static __device__ __forceinline__ v16f mfma_mx4_32(const int4 &
 
 template <int FM, int FN, int WM, int WN, int STAGES> struct tile_shape {
     static constexpr int TM = 32 * FM * WM, TN = 32 * FN * WN, NW = WM * WN;
-    static constexpr int CODES = (TM + TN) * 64, STAGE = CODES + (TM + TN) * 4, LDS = STAGES * STAGE;
-    static constexpr int CI = (TM + TN) / 16;   // 1-KiB copies of a panel's codes: 16 rows each
-    static constexpr int SI = (TM + TN) / 64;   // 256-B copies of its exponents: 64 rows each
-    static_assert(CI % NW == 0 && SI % NW == 0, "every wave issues the same copies");
+    static constexpr int CODES = (TM + TN) * 128, STAGE = CODES + (TM + TN) * 8, LDS = STAGES * STAGE;
+    static constexpr int CI = (TM + TN) / 8;    // 1-KiB copies of a plane's codes: 8 rows each
+    static constexpr int SI = (TM + TN) / 32;   // 256-B copies of its exponents: 32 rows each
+    static_assert(CI % NW == 0 && SI % NW == 0 && NW % 2 == 0, "every wave issues the same copies");
 };
 
 // the fragments of one step: FM of the weights, FN of x
@@ -54,8 +54,8 @@ template <int FM, int FN> struct frags {
     // one of the FM + FN reads; the first instructions want a[0] and b[0]
     template <int I> __device__ __forceinline__ void load(const char * ca, const char * cb) {
         if constexpr (I == 0) a[0] = *(const int4 *) ca;
-        else if constexpr (I <= FN) b[I - 1] = *(const int4 *) (cb + (I - 1) * 32 * 64);
-        else a[I - FN] = *(const int4 *) (ca + (I - FN) * 32 * 64);
+        else if constexpr (I <= FN) b[I - 1] = *(const int4 *) (cb + (I - 1) * 32 * 128);
+        else a[I - FN] = *(const int4 *) (ca + (I - FN) * 32 * 128);
     }
 };
 
@@ -130,54 +130,59 @@ static __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tile(mx4_args a, un
     };
 #pragma unroll
     for (int k = 0; k < CK; ++k) {
-        const int r = (wave + k * S::NW) * 16 + (lane >> 2);
+        const int r = (wave + k * S::NW) * 8 + (lane >> 3);
         code_row[k] = (r < S::TM ? wc : a.x_codes) + source(r) * a.KB * 16;
     }
 #pragma unroll
     for (int k = 0; k < COPIES - CK; ++k) {
-        const int r = (wave + k * S::NW) * 64 + lane;
-        exp_row[k] = (r < S::TM ? ws : a.x_scales) + source(r) * 8;
+        const int r = (wave + k * S::NW) * 32 + (lane >> 1);
+        exp_row[k] = (r < S::TM ? ws : a.x_scales) + source(r) * 8 + (lane & 1) * 4;
         exp_step[k] = (r < S::TM ? a.M : a.x_rows) * 8;
     }
     const unsigned lds0 = (unsigned) (uintptr_t) (lds_char *) lds;
-    const int blk = (lane & 3) ^ (lane >> 4);   // the block that this lane copies
-    const int last = (a.KB + 3) / 4 - 1;
-    // copy c of panel h into its place in the ring; past the last panel that one comes again, into a
+    // the block that this lane copies: its rows are 8 (wave + k NW) + lane / 8, NW even
+    const int blk = (lane & 7) ^ ((wave & 1) * 4 + (lane >> 4));
+    const int last = (a.KB + 7) / 8 - 1;
+    // copy c of plane h into its place in the ring; past the last plane that one comes again, into a
     // place that nothing reads any more, so that the number of copies on their way is always known
     auto copy = [&](int h, auto cc) {
         constexpr int c = cc;
         const unsigned to = lds0 + h % STAGES * S::STAGE;
         const int p = min(h, last);
-        if constexpr (c < CK) dma16(code_row[c] + (int64_t) min(p * 4 + blk, a.KB - 1) * 16, to + (wave + c * S::NW) * 1024);
-        else dma4(exp_row[c - CK] + (p >> 1) * exp_step[c - CK] + (p & 1) * 4, to + S::CODES + (wave + (c - CK) * S::NW) * 256);
+        if constexpr (c < CK) dma16(code_row[c] + (int64_t) min(p * 8 + blk, a.KB - 1) * 16, to + (wave + c * S::NW) * 1024);
+        else dma4(exp_row[c - CK] + p * exp_step[c - CK], to + S::CODES + (wave + (c - CK) * S::NW) * 256);
     };
 
     const int wm = wave % WM * 32 * FM, wn = S::TM + wave / WM * 32 * FN;
     const int r31 = lane & 31, half = lane >> 5;
-    const char * ca = lds + (wm + r31) * 64, * cb = lds + (wn + r31) * 64;
-    const char * ea = lds + S::CODES + (wm + r31) * 4, * eb = lds + S::CODES + (wn + r31) * 4;
-    const int slot[2] = {((2 * half) ^ (r31 >> 2 & 3)) * 16, ((2 * half + 1) ^ (r31 >> 2 & 3)) * 16};
+    const char * ca = lds + (wm + r31) * 128, * cb = lds + (wn + r31) * 128;
+    const char * ea = lds + S::CODES + (wm + r31) * 8 + half * 4, * eb = lds + S::CODES + (wn + r31) * 8 + half * 4;
+    int slot[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) slot[j] = ((j + 4 * half) ^ (r31 >> 1 & 7)) * 16;
     int sa[FM], sb[FN], na[FM], nb[FN];
     auto load_exps = [&](int at) {
 #pragma unroll
-        for (int i = 0; i < FM; ++i) na[i] = *(const int *) (ea + at + i * 32 * 4);
+        for (int i = 0; i < FM; ++i) na[i] = *(const int *) (ea + at + i * 32 * 8);
 #pragma unroll
-        for (int i = 0; i < FN; ++i) nb[i] = *(const int *) (eb + at + i * 32 * 4);
+        for (int i = 0; i < FN; ++i) nb[i] = *(const int *) (eb + at + i * 32 * 8);
     };
-    auto take_exps = [&](int h) {   // this lane's two blocks', 0 past K
-        const unsigned width = 8 * min(max(a.KB - h * 4 - 2 * half, 0), 2);
+    auto take_exps = [&](int h) {   // this lane's four blocks', 0 past K
+        const int left = min(max(a.KB - h * 8 - 4 * half, 0), 4);
+        const int mask = left == 4 ? ~0 : (1 << (8 * left)) - 1;
 #pragma unroll
-        for (int i = 0; i < FM; ++i) sa[i] = (int) __builtin_amdgcn_ubfe((unsigned) na[i], 16u * half, width);
+        for (int i = 0; i < FM; ++i) sa[i] = na[i] & mask;
 #pragma unroll
-        for (int i = 0; i < FN; ++i) sb[i] = (int) __builtin_amdgcn_ubfe((unsigned) nb[i], 16u * half, width);
+        for (int i = 0; i < FN; ++i) sb[i] = nb[i] & mask;
     };
 
-    // A step's fragments are read between the instructions of the one before.  Before a panel's
-    // second step all waves have read its place and the next panel has come: the barrier stands
-    // there.  Then the next panel's first fragments are read, and panel h + STAGES is copied to the
-    // free place during this step and the next panel's first one.
+    // A step's fragments are read between the instructions of the one before.  Before a plane's last
+    // step all waves have read its place and the next plane has come: the barrier stands there.  Then
+    // the next plane's first fragments are read, and plane h + STAGES is copied to the free place
+    // during this step (part 0) and the next plane's first two (parts 1 and 2), spread over their
+    // instructions: all at once they would hold up the wave that issues them.
     constexpr int INS = FM * FN, FR = FM + FN, PER = (FR + INS - 1) / INS, EVERY = INS / FR > 0 ? INS / FR : 1;
-    constexpr int AHEAD = (STAGES - 2) * COPIES;   // copies of later panels on their way at the barrier
+    constexpr int AHEAD = (STAGES - 2) * COPIES;   // copies of later planes on their way at the barrier
     v16f acc[FM][FN] = {};
     frags<FM, FN> f0, f1;
     auto reads = [&](frags<FM, FN> & f, int at, int j, auto i) {
@@ -187,39 +192,45 @@ static __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tile(mx4_args a, un
                 if constexpr (n < FR) f.template load<n>(ca + at + slot[j], cb + at + slot[j]);
             });
     };
-    auto copies = [&](int h, auto step, auto i) {   // evenly over the 2 INS instructions of both steps
+    auto copies = [&](int h, auto part, auto i) {   // those in front of instruction i of part's step
         unroll<COPIES>([&](auto c) {
-            if constexpr ((c * 2 + 1) * INS / COPIES == step * INS + i) copy(h, c);
+            if constexpr ((c * 2 + 1) * 3 * INS / (2 * COPIES) == part * INS + i) copy(h, c);
         });
     };
-    constexpr std::integral_constant<int, 0> FIRST{};
-    constexpr std::integral_constant<int, 1> SECOND{};
+    constexpr std::integral_constant<int, 0> P0{};
+    constexpr std::integral_constant<int, 1> P1{};
+    constexpr std::integral_constant<int, 2> P2{};
     for (int h = 0; h < STAGES - 1; ++h) unroll<COPIES>([&](auto c) { copy(h, c); });
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(AHEAD) : "memory");
-    unroll<INS>([&](auto i) { copies(STAGES - 1, FIRST, i); });
+    unroll<INS>([&](auto i) { copies(STAGES - 1, P0, i); });
     // a wave whose part of the tile lies past M or the tile's rows only copies: its results are not
     // stored, and the others have the matrix cores to themselves
     if (m0 + wm >= a.M || wn - S::TM >= tr.n) {
         for (int h = 0; h < last; ++h) {
-            unroll<INS>([&](auto i) { copies(h + STAGES - 1, SECOND, i); });
+            unroll<INS>([&](auto i) { copies(h + STAGES - 1, P1, i); });
+            unroll<INS>([&](auto i) { copies(h + STAGES - 1, P2, i); });
             asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(AHEAD) : "memory");
-            unroll<INS>([&](auto i) { copies(h + STAGES, FIRST, i); });
+            unroll<INS>([&](auto i) { copies(h + STAGES, P0, i); });
         }
     } else {
-    unroll<FR>([&](auto i) { f0.template load<i>(ca + slot[0], cb + slot[0]); });
-    load_exps(0);
-    take_exps(0);
-    int at = 0;
-    for (int h = 0; h < last; ++h) {
-        mma_step<0>(acc, f0, sa, sb, [&](auto i) { reads(f1, at, 1, i); copies(h + STAGES - 1, SECOND, i); });
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(AHEAD) : "memory");
-        at = at + S::STAGE == S::LDS ? 0 : at + S::STAGE;
-        load_exps(at);
-        mma_step<1>(acc, f1, sa, sb, [&](auto i) { reads(f0, at, 0, i); copies(h + STAGES, FIRST, i); });
-        take_exps(h + 1);
-    }
-    mma_step<0>(acc, f0, sa, sb, [&](auto i) { reads(f1, at, 1, i); });
-    mma_step<1>(acc, f1, sa, sb, [](auto) {});
+        unroll<FR>([&](auto i) { f0.template load<i>(ca + slot[0], cb + slot[0]); });
+        load_exps(0);
+        take_exps(0);
+        int at = 0;
+        for (int h = 0; h < last; ++h) {
+            mma_step<0>(acc, f0, sa, sb, [&](auto i) { reads(f1, at, 1, i); copies(h + STAGES - 1, P1, i); });
+            mma_step<1>(acc, f1, sa, sb, [&](auto i) { reads(f0, at, 2, i); copies(h + STAGES - 1, P2, i); });
+            mma_step<2>(acc, f0, sa, sb, [&](auto i) { reads(f1, at, 3, i); });
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(AHEAD) : "memory");
+            at = at + S::STAGE == S::LDS ? 0 : at + S::STAGE;
+            load_exps(at);
+            mma_step<3>(acc, f1, sa, sb, [&](auto i) { reads(f0, at, 0, i); copies(h + STAGES, P0, i); });
+            take_exps(h + 1);
+        }
+        mma_step<0>(acc, f0, sa, sb, [&](auto i) { reads(f1, at, 1, i); });
+        mma_step<1>(acc, f1, sa, sb, [&](auto i) { reads(f0, at, 2, i); });
+        mma_step<2>(acc, f0, sa, sb, [&](auto i) { reads(f1, at, 3, i); });
+        mma_step<3>(acc, f1, sa, sb, [](auto) {});
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no copy is left when the shared memory gets another use
 
@@ -278,27 +289,33 @@ static hipError_t run_tile(const mx4_args & a, int ytype, hipStream_t st) {
     });
 }
 
-// Which tile: the one whose time, by what a CU was measured to take (us), comes out least.  A panel
-// (128 of K) of a 256 x 256 tile takes 1.0 (one workgroup a CU), of a 128 x 128 tile 0.32 alone and
-// 0.4 each of more (two at a time), of a 64 x 64 tile 0.19 alone and 0.17 each of more (four at a
-// time); beginning and end add 8, 4 and 4.  Large tiles move the least bytes for their products, small
-// ones give more CUs work: 512 x 28672 x 4096 takes 40 / 60 / 86 us, 1024 x 4096 x 4096 26 / 16 / 23,
-// 256 x 4096 x 4096 25 / 14 / 10.
+// Which tile: the one whose time, by what a CU was measured to take (us), comes out least.  A plane
+// (256 of K) takes 2.1 in a 256 x 256 tile, 0.65 in a 128 x 128 tile alone on its CU and 0.8 in one of
+// several, 0.33 and 0.26 in 64 x 64 tiles; beginning and end add 8, 4 and 4.  Tiles come in whole rounds
+// of the CUs; experts' are counted as half full at their ends, a quarter of a tile each, since waves
+// without rows cost little, and the routing's rounds as half one more.  Large tiles move the least
+// bytes for their products, small ones give more CUs work: 512 x 28672 x 4096 takes 38 us in tiles of
+// 256 and 50 in tiles of 128, 1024 x 4096 x 4096 25 and 15, 256 x 4096 x 4096 24 and 14, in tiles of 64 9.5;
+// 8192 pairs by 8 experts of 4096 x 14336 335 in tiles of 256, 382 in tiles of 128.
+// Deep rings serve CUs that have one tile (512 x 4096 x 14336: 38 us with four planes, 58 with two),
+// shallow ones let several share a CU (2048 x 4096 x 4096: 27 and 24; experts' tiles of 64, 300 tokens
+// by 8 experts of 4096 x 4096: 24 and 20).
 template <bool IDS> static hipError_t pick_tile(const mx4_args & a, int ytype, hipStream_t st) {
     constexpr double CUS = 256;
-    const double panels = (a.KB + 3) / 4;
+    const double planes = (a.KB + 7) / 8;
     auto load = [&](int side) {   // tiles per CU
         const int64_t busy = a.T < a.n_expert ? a.T : a.n_expert;
-        const double n = IDS ? (double) a.T / side + 0.5 * busy : (double) ((a.T + side - 1) / side);
+        const double n = IDS ? (double) a.T / side + 0.25 * busy : (double) ((a.T + side - 1) / side);
         return n * ((a.M + side - 1) / side) / CUS;
     };
+    auto rounds = [](double n) { return IDS ? std::max(n + 0.5, 1.0) : std::ceil(n); };
     const double n256 = load(256), n128 = load(128), n64 = load(64);
-    const double t256 = std::ceil(n256) * (panels * 1.0 + 8);
-    const double t128 = n128 <= 1 ? panels * 0.32 + 4 : std::ceil(n128) * (panels * 0.4 + 4);
-    const double t64 = n64 <= 1 ? panels * 0.19 + 4 : std::ceil(n64) * panels * 0.17 + std::ceil(n64 / 4) * 4;
-    if (t256 <= t128 && t256 <= t64) return run_tile<4, 2, 2, 4, 4, IDS>(a, ytype, st);
-    if (t128 <= t64) return run_tile<2, 2, 2, 2, 4, IDS>(a, ytype, st);
-    return run_tile<1, 2, 2, 1, 4, IDS>(a, ytype, st);
+    const double t256 = rounds(n256) * (planes * 2.1 + 8);
+    const double t128 = n128 <= 1 ? rounds(n128) * (planes * 0.65 + 4) : rounds(n128) * planes * 0.8 + rounds(n128 / 2) * 4;
+    const double t64 = n64 <= 1 ? rounds(n64) * (planes * 0.33 + 4) : rounds(n64) * planes * 0.26 + rounds(n64 / 4) * 4;
+    if (t256 <= t128 && t256 <= t64) return run_tile<4, 2, 2, 4, 2, IDS>(a, ytype, st);
+    if (t128 <= t64) return n128 <= 1 ? run_tile<2, 2, 2, 2, 4, IDS>(a, ytype, st) : run_tile<2, 2, 2, 2, 2, IDS>(a, ytype, st);
+    return run_tile<1, 2, 2, 1, IDS ? 2 : 4, IDS>(a, ytype, st);
 }
 
 hipError_t mx4_product_tile(const mx4_args & a, int ytype, hipStream_t st) {
