@@ -157,15 +157,17 @@ int mi355x_mx4_quantize(int xtype, const void * x, int64_t ldx, int64_t rows, in
                         void * stream);
 int mi355x_mx4_dequantize(const uint8_t * codes, const uint8_t * scales, int64_t rows, int64_t K, int ytype, void * y,
                           void * stream);
-// y[T][M] = W[M][K] . x[T][K], W in MXFP4.  x as MXFP4 (xtype MI355X_MX4: x its codes, x_scales), or
-// as f32 / f16 / bf16 rows that the call quantises into the workspace first; sums in f32
-int64_t mi355x_mx4_mul_mat_workspace(int64_t T, int64_t K);
+// y[T][M] = W[M][K] . x[T][K], W in MXFP4.  x as MXFP4 (xtype MI355X_MX4: x its codes, x_scales; ldx is
+// not looked at), or as f32 / f16 / bf16 rows that the call quantises first; sums in f32.  work: as many
+// bytes as the workspace call says, for quantised rows and for sums of shares of K
+int64_t mi355x_mx4_mul_mat_workspace(int64_t M, int64_t K, int xtype, int64_t T);
 int mi355x_mx4_mul_mat(const uint8_t * w_codes, const uint8_t * w_scales, int64_t M, int64_t K, int xtype, const void * x,
                        const uint8_t * x_scales, int64_t ldx, int64_t T, int ytype, void * y, void * work, int64_t work_bytes,
                        void * stream);
 // the experts' product on sorted pairs: y[p][M] = W[e][M][K] . x for offsets[e] <= p < offsets[e + 1],
 // with x row order[p] / used of x[T][K], or with x_sorted row p of x[T * used][K]; rows from
-// offsets[n_expert] on are set to zero.  The workspace is mi355x_mx4_mul_mat_workspace of x's rows
+// offsets[n_expert] on are set to zero
+int64_t mi355x_mx4_mul_mat_id_workspace(int64_t M, int64_t K, int64_t n_expert, int xtype, int64_t T, int64_t used, int x_sorted);
 int mi355x_mx4_mul_mat_id(const uint8_t * w_codes, const uint8_t * w_scales, int64_t M, int64_t K, int64_t n_expert, int xtype,
                           const void * x, const uint8_t * x_scales, int64_t ldx, int64_t T, int64_t used, int x_sorted,
                           const int32_t * order, const int32_t * offsets, int ytype, void * y, void * work,

@@ -43,12 +43,14 @@ struct moe_view {
 hipError_t mx4_quantize(int type, const void * x, int64_t ldx, int64_t rows, int64_t K, uint8_t * codes, uint8_t * scales,
                         hipStream_t st);
 hipError_t mx4_dequantize(const mx4_mat & m, int type, void * y, hipStream_t st);
-// y [T][M] = W . x for MXFP4 rows x
-hipError_t mx4_product(const mx4_mat & w, const mx4_mat & x, int ytype, void * y, hipStream_t st);
-// y [pairs][M]: sorted row p is expert e(p)'s W times x row order[p] / used (or p)
-hipError_t mx4_product_id(const mx4_mat & w, const mx4_mat & x, const moe_view & v, int ytype, void * y, hipStream_t st);
-// few rows of floats, quantised where they are used: whether that is the way for them, and the product
-bool mx4_takes_floats(const mx4_mat & w, int64_t x_rows, const moe_view * v);
+// y [T][M] = W . x, or by experts with a view: sorted row p of y [pairs][M] is expert e(p)'s W times x
+// row order[p] / used (or p)
+struct mx4_needs {
+    bool quantized;   // x has to come as MXFP4; few rows of floats go to mx4_product_float
+    int64_t part;     // bytes of workspace for sums, beside x's
+};
+mx4_needs mx4_product_needs(const mx4_mat & w, int64_t x_rows, const moe_view * v);
+hipError_t mx4_product(const mx4_mat & w, const mx4_mat & x, const moe_view * v, int ytype, void * y, void * part, hipStream_t st);
 hipError_t mx4_product_float(const mx4_mat & w, int xtype, const void * x, int64_t ldx, int64_t x_rows, const moe_view * v,
                              int ytype, void * y, hipStream_t st);
 

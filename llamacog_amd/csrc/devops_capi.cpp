@@ -99,71 +99,84 @@ OPS_API int mi355x_mx4_dequantize(const uint8_t * codes, const uint8_t * scales,
     return cs.done(mx4_dequantize({codes, scales, rows, K}, ytype, y, cs.st));
 }
 
-OPS_API int64_t mi355x_mx4_mul_mat_workspace(int64_t T, int64_t K) {
-    return check_rows(T, K) ? -1 : codes_bytes(T, K) + scales_bytes(T, K);
-}
+// a product's arguments, checked; x_rows rows of x
+struct product {
+    mx4_mat w;
+    int xtype;
+    const void * x;
+    const uint8_t * x_scales;
+    int64_t ldx, x_rows;
+    const moe_view * view;
+    int ytype;
+    void * y;
 
-// the x operand of a product: MXFP4 as given, or quantised into the workspace
-static int x_operand(int xtype, const void * x, const uint8_t * xscales, int64_t ldx, int64_t rows, int64_t K, void * work,
-                     hipStream_t st, mx4_mat & m) {
-    if (xtype == MI355X_MX4) {
-        m = {(const uint8_t *) x, xscales, rows, K};
-        return 0;
+    int64_t x_bytes() const { return codes_bytes(x_rows, w.K) + (scales_bytes(x_rows, w.K) + 255) / 256 * 256; }
+
+    int64_t workspace() const {
+        const mx4_needs n = mx4_product_needs(w, x_rows, view);
+        return (xtype != MI355X_MX4 && n.quantized ? x_bytes() : 0) + n.part;
     }
-    uint8_t * codes = (uint8_t *) work, * scales = codes + codes_bytes(rows, K);
-    m = {codes, scales, rows, K};
-    return mx4_quantize(xtype, x, ldx, rows, K, codes, scales, st) == hipSuccess ? 0 : MI355X_ERR_HIP;
-}
 
-static int check_x(int xtype, const void * x, const uint8_t * xscales, int64_t ldx, int64_t rows, int64_t K, const void * work,
-                   int64_t work_bytes) {
-    TRY(check_rows(rows, K));
-    if (xtype == MI355X_MX4) return check_mx4(x, xscales);
-    TRY(check_elems(xtype, x));
-    if (ldx < K && rows > 1) return MI355X_ERR_SHAPE;
-    if (!aligned(work, 16)) return MI355X_ERR_ALIGN;
-    return work_bytes >= codes_bytes(rows, K) + scales_bytes(rows, K) ? 0 : MI355X_ERR_WORKSPACE;
+    int check_shape() const {
+        TRY(check_rows(w.rows, w.K));
+        TRY(check_rows(x_rows, w.K));
+        return xtype == MI355X_MX4 || is_elem(xtype) ? 0 : MI355X_ERR_TYPE;
+    }
+
+    int run(void * work, int64_t work_bytes, void * stream) const {
+        TRY(check_shape());
+        TRY(check_mx4(w.codes, w.scales));
+        if (xtype == MI355X_MX4) TRY(check_mx4(x, x_scales));
+        else TRY(check_elems(xtype, x));
+        if (xtype != MI355X_MX4 && ldx < w.K && x_rows > 1) return MI355X_ERR_SHAPE;
+        TRY(check_elems(ytype, y));
+        if (!aligned(work, 16)) return MI355X_ERR_ALIGN;
+        if (x_rows == 0 || w.rows == 0) return 0;
+        if (work_bytes < workspace()) return MI355X_ERR_WORKSPACE;
+        call_stream cs(stream);
+        if (cs.err != hipSuccess) return MI355X_ERR_HIP;
+        if (xtype == MI355X_MX4)
+            return cs.done(mx4_product(w, {(const uint8_t *) x, x_scales, x_rows, w.K}, view, ytype, y, work, cs.st));
+        if (!mx4_product_needs(w, x_rows, view).quantized)
+            return cs.done(mx4_product_float(w, xtype, x, ldx, x_rows, view, ytype, y, cs.st));
+        uint8_t * codes = (uint8_t *) work, * scales = codes + codes_bytes(x_rows, w.K);
+        const hipError_t e = mx4_quantize(xtype, x, ldx, x_rows, w.K, codes, scales, cs.st);
+        if (e != hipSuccess) return cs.done(e);
+        return cs.done(mx4_product(w, {codes, scales, x_rows, w.K}, view, ytype, y, codes + x_bytes(), cs.st));
+    }
+};
+
+static int check_experts(int64_t n_expert) { return n_expert > 0 && n_expert <= MOE_MAX_EXPERTS ? 0 : MI355X_ERR_SHAPE; }
+
+OPS_API int64_t mi355x_mx4_mul_mat_workspace(int64_t M, int64_t K, int xtype, int64_t T) {
+    const product p = {{nullptr, nullptr, M, K}, xtype, nullptr, nullptr, K, T, nullptr, ELEM_F32, nullptr};
+    return p.check_shape() ? -1 : T == 0 || M == 0 ? 0 : p.workspace();
 }
 
 OPS_API int mi355x_mx4_mul_mat(const uint8_t * w_codes, const uint8_t * w_scales, int64_t M, int64_t K, int xtype,
                                const void * x, const uint8_t * x_scales, int64_t ldx, int64_t T, int ytype, void * y,
                                void * work, int64_t work_bytes, void * stream) {
-    TRY(check_rows(M, K));
-    TRY(check_mx4(w_codes, w_scales));
-    TRY(check_x(xtype, x, x_scales, ldx, T, K, work, work_bytes));
-    TRY(check_elems(ytype, y));
-    if (T == 0 || M == 0) return 0;
-    call_stream cs(stream);
-    if (cs.err != hipSuccess) return MI355X_ERR_HIP;
-    const mx4_mat w = {w_codes, w_scales, M, K};
-    if (xtype != MI355X_MX4 && mx4_takes_floats(w, T, nullptr))
-        return cs.done(mx4_product_float(w, xtype, x, ldx, T, nullptr, ytype, y, cs.st));
-    mx4_mat xm;
-    TRY(x_operand(xtype, x, x_scales, ldx, T, K, work, cs.st, xm));
-    return cs.done(mx4_product(w, xm, ytype, y, cs.st));
+    const product p = {{w_codes, w_scales, M, K}, xtype, x, x_scales, ldx, T, nullptr, ytype, y};
+    return p.run(work, work_bytes, stream);
+}
+
+OPS_API int64_t mi355x_mx4_mul_mat_id_workspace(int64_t M, int64_t K, int64_t n_expert, int xtype, int64_t T, int64_t used,
+                                                int x_sorted) {
+    if (check_routing(T, used) || check_experts(n_expert)) return -1;
+    const moe_view v = {nullptr, nullptr, T * used, (int) n_expert, x_sorted ? 0 : (int) used};
+    const product p = {{nullptr, nullptr, M, K}, xtype, nullptr, nullptr, K, x_sorted ? T * used : T, &v, ELEM_F32, nullptr};
+    return p.check_shape() ? -1 : T == 0 || M == 0 ? 0 : p.workspace();
 }
 
 OPS_API int mi355x_mx4_mul_mat_id(const uint8_t * w_codes, const uint8_t * w_scales, int64_t M, int64_t K, int64_t n_expert,
                                   int xtype, const void * x, const uint8_t * x_scales, int64_t ldx, int64_t T, int64_t used,
                                   int x_sorted, const int32_t * order, const int32_t * offsets, int ytype, void * y,
                                   void * work, int64_t work_bytes, void * stream) {
-    TRY(check_rows(M, K));
-    TRY(check_mx4(w_codes, w_scales));
     TRY(check_routing(T, used));
-    if (n_expert <= 0 || n_expert > MOE_MAX_EXPERTS) return MI355X_ERR_SHAPE;
-    const int64_t rows = x_sorted ? T * used : T;
-    TRY(check_x(xtype, x, x_scales, ldx, rows, K, work, work_bytes));
-    TRY(check_elems(ytype, y));
-    if (T == 0 || M == 0) return 0;
-    call_stream cs(stream);
-    if (cs.err != hipSuccess) return MI355X_ERR_HIP;
-    const mx4_mat w = {w_codes, w_scales, M, K};
+    TRY(check_experts(n_expert));
     const moe_view v = {order, offsets, T * used, (int) n_expert, x_sorted ? 0 : (int) used};
-    if (xtype != MI355X_MX4 && mx4_takes_floats(w, rows, &v))
-        return cs.done(mx4_product_float(w, xtype, x, ldx, rows, &v, ytype, y, cs.st));
-    mx4_mat xm;
-    TRY(x_operand(xtype, x, x_scales, ldx, rows, K, work, cs.st, xm));
-    return cs.done(mx4_product_id(w, xm, v, ytype, y, cs.st));
+    const product p = {{w_codes, w_scales, M, K}, xtype, x, x_scales, ldx, x_sorted ? T * used : T, &v, ytype, y};
+    return p.run(work, work_bytes, stream);
 }
 
 OPS_API int64_t mi355x_moe_sort_workspace(int64_t T, int64_t used, int64_t n_expert) {

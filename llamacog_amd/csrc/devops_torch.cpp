@@ -156,27 +156,37 @@ struct operand {
     int type;
     int64_t rows, step;
     const uint8_t * scales;
-    Tensor work;
     at::ScalarType out;   // unless the caller asks for another
 };
 
 operand check_operand(const Tensor & x, const std::optional<Tensor> & x_scales, const Tensor & w, int64_t k) {
-    operand o;
     beside(x, "x", w);
+    operand o;
     int64_t have;
     if (x_scales) {
         const mx4 m = check_mx4(x, *x_scales, "x", 2);
-        o = {MI355X_MX4, m.rows, m.k, bytes(*x_scales), Tensor(), at::kFloat};
+        o = {MI355X_MX4, m.rows, m.k, bytes(*x_scales), at::kFloat};
         have = m.k;
     } else {
         const int type = matrix(x, "x");
-        o = {type, x.size(0), row_step(x), nullptr, Tensor(), x.scalar_type()};
+        o = {type, x.size(0), row_step(x), nullptr, x.scalar_type()};
         have = x.size(1);
     }
     TORCH_CHECK_VALUE(have == k, "x: rows of ", k, " elements are wanted, got ", have);
-    if (!x_scales) o.work = fresh({mi355x_mx4_mul_mat_workspace(o.rows, k)}, x, at::kByte);
     return o;
 }
+
+struct workspace {
+    Tensor t;
+    void * p = nullptr;
+    int64_t size;
+    workspace(int64_t size, const Tensor & like) : size(size) {
+        if (size > 0) {
+            t = fresh({size}, like, at::kByte);
+            p = t.mutable_data_ptr();
+        }
+    }
+};
 
 Tensor mul_mat(const Tensor & w_codes, const Tensor & w_scales, const Tensor & x, const std::optional<Tensor> & x_scales,
                std::optional<at::ScalarType> dtype) {
@@ -185,10 +195,10 @@ Tensor mul_mat(const Tensor & w_codes, const Tensor & w_scales, const Tensor & x
     const at::ScalarType out = dtype.value_or(o.out);
     const int ytype = elem_type(out, "dtype");
     Tensor y = fresh({o.rows, w.rows}, w_codes, out);
+    const workspace work(mi355x_mx4_mul_mat_workspace(w.rows, w.k, o.type, o.rows), w_codes);
     launch on(w_codes);
     check(mi355x_mx4_mul_mat(bytes(w_codes), bytes(w_scales), w.rows, w.k, o.type, x.const_data_ptr(), o.scales, o.step, o.rows,
-                             ytype, y.mutable_data_ptr(), o.work.defined() ? o.work.mutable_data_ptr() : nullptr,
-                             o.work.defined() ? o.work.numel() : 0, on.stream), "mx4_mul_mat");
+                             ytype, y.mutable_data_ptr(), work.p, work.size, on.stream), "mx4_mul_mat");
     return y;
 }
 
@@ -204,11 +214,11 @@ Tensor mul_mat_id(const Tensor & w_codes, const Tensor & w_scales, const Tensor 
     const at::ScalarType out = dtype.value_or(o.out);
     const int ytype = elem_type(out, "dtype");
     Tensor y = fresh({p.t * p.used, w.rows}, w_codes, out);
+    const workspace work(mi355x_mx4_mul_mat_id_workspace(w.rows, w.k, p.experts, o.type, p.t, p.used, x_sorted), w_codes);
     launch on(w_codes);
     check(mi355x_mx4_mul_mat_id(bytes(w_codes), bytes(w_scales), w.rows, w.k, p.experts, o.type, x.const_data_ptr(), o.scales,
-                                o.step, p.t, p.used, x_sorted, ints(order), ints(offsets), ytype, y.mutable_data_ptr(),
-                                o.work.defined() ? o.work.mutable_data_ptr() : nullptr,
-                                o.work.defined() ? o.work.numel() : 0, on.stream), "mx4_mul_mat_id");
+                                o.step, p.t, p.used, x_sorted, ints(order), ints(offsets), ytype, y.mutable_data_ptr(), work.p,
+                                work.size, on.stream), "mx4_mul_mat_id");
     return y;
 }
 
@@ -221,13 +231,11 @@ std::tuple<Tensor, Tensor, Tensor> sort(const Tensor & ids, int64_t n_expert) {
     const int64_t t = ids.size(0), used = ids.size(1);
     check_routing(used, n_expert);
     Tensor order = fresh({t * used}, ids, at::kInt), rank = fresh({t, used}, ids, at::kInt), offsets = fresh({n_expert + 1}, ids, at::kInt);
-    const int64_t size = mi355x_moe_sort_workspace(t, used, n_expert);
-    Tensor work;
-    if (size > 0) work = fresh({size}, ids, at::kByte);
+    const workspace work(mi355x_moe_sort_workspace(t, used, n_expert), ids);
     launch on(ids);
     check(mi355x_moe_sort(ids.const_data_ptr(), (int) ids.element_size(), t, used, n_expert, (int32_t *) order.mutable_data_ptr(),
                           (int32_t *) rank.mutable_data_ptr(), (int32_t *) offsets.mutable_data_ptr(),
-                          work.defined() ? work.mutable_data_ptr() : nullptr, size, on.stream), "moe_sort");
+                          work.p, work.size, on.stream), "moe_sort");
     return {order, rank, offsets};
 }
 

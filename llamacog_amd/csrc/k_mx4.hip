@@ -278,7 +278,7 @@ static hipError_t run_mv(const mx4_args & a, const X * x, int64_t ldx, int ytype
     });
 }
 
-static mx4_args product_args(const mx4_mat & w, const mx4_mat & x, void * y) {
+static mx4_args product_args(const mx4_mat & w, const mx4_mat & x, const moe_view * v, void * y) {
     mx4_args a{};
     a.w_codes = w.codes;
     a.w_scales = w.scales;
@@ -289,54 +289,47 @@ static mx4_args product_args(const mx4_mat & w, const mx4_mat & x, void * y) {
     a.x_codes = x.codes;
     a.x_scales = x.scales;
     a.x_rows = x.rows;
-    a.T = x.rows;
+    a.T = v ? v->pairs : x.rows;
     a.y = y;
+    if (v) {
+        a.order = v->order;
+        a.offsets = v->offsets;
+        a.n_expert = v->n_expert;
+        a.used = v->used;
+    }
     return a;
 }
 
-static mx4_args id_args(const mx4_mat & w, const mx4_mat & x, const moe_view & v, void * y) {
-    mx4_args a = product_args(w, x, y);
-    a.order = v.order;
-    a.offsets = v.offsets;
-    a.n_expert = v.n_expert;
-    a.used = v.used;
-    a.T = v.pairs;
-    return a;
+// The kernel for few rows, as long as its tiles of 16 or 32 rows read the weights about once: 4096 x
+// 4096 by 20 rows takes 5.6 us here and 9.2 in 64 x 64 tiles, 28672 x 4096 by 64 rows 28.6 and 18.5;
+// by experts up to 16 rows each.
+static bool few_rows(const mx4_args & a) {
+    return a.T <= (a.n_expert ? 16 * (int64_t) a.n_expert : 32) && mv_lds(a, 1, MV_WAVES) <= MV_LDS;
 }
 
-// The kernel for few rows as long as its tiles of 16 or 32 rows read the weights about once: 4096 x
-// 4096 by 20 rows takes 5.6 us here and 9.2 in 64 x 64 tiles, 28672 x 4096 by 64 rows 28.6 and 18.5.
-static bool few_rows(const mx4_args & a, int64_t rows, int64_t most) { return rows <= most && mv_lds(a, 1, MV_WAVES) <= MV_LDS; }
+// few enough that every workgroup may quantise those of its tile
+static bool float_rows(const mx4_args & a) { return few_rows(a) && a.T <= (a.n_expert ? 16 : 2); }
 
-hipError_t mx4_product(const mx4_mat & w, const mx4_mat & x, int ytype, void * y, hipStream_t st) {
-    const mx4_args a = product_args(w, x, y);
+mx4_needs mx4_product_needs(const mx4_mat & w, int64_t x_rows, const moe_view * v) {
+    const mx4_args a = product_args(w, {nullptr, nullptr, x_rows, w.K}, v, nullptr);
+    return {!float_rows(a), few_rows(a) ? 0 : mx4_tile_workspace(a)};
+}
+
+hipError_t mx4_product(const mx4_mat & w, const mx4_mat & x, const moe_view * v, int ytype, void * y, void * part, hipStream_t st) {
+    const mx4_args a = product_args(w, x, v, y);
     const mxfp4 * in = nullptr;
-    if (!few_rows(a, a.T, 32)) return mx4_product_tile(a, ytype, st);
+    if (!few_rows(a)) return mx4_product_tile(a, (float *) part, ytype, st);
+    if (v) return run_mv<1, mxfp4, true>(a, in, 0, ytype, st);
     if (a.T > 16 && mv_lds(a, 2, MV_WAVES) <= MV_LDS) return run_mv<2, mxfp4, false>(a, in, 0, ytype, st);
     return run_mv<1, mxfp4, false>(a, in, 0, ytype, st);
 }
 
-hipError_t mx4_product_id(const mx4_mat & w, const mx4_mat & x, const moe_view & v, int ytype, void * y, hipStream_t st) {
-    const mx4_args a = id_args(w, x, v, y);
-    const mxfp4 * in = nullptr;
-    if (!few_rows(a, v.pairs, 16 * (int64_t) v.n_expert)) return mx4_product_tile(a, ytype, st);   // 16 rows an expert
-    return run_mv<1, mxfp4, true>(a, in, 0, ytype, st);
-}
-
-bool mx4_takes_floats(const mx4_mat & w, int64_t x_rows, const moe_view * v) {
-    const mx4_mat x = {nullptr, nullptr, x_rows, w.K};
-    // few enough that every workgroup may quantise those of its tile
-    if (!v) return few_rows(product_args(w, x, nullptr), x_rows, 2);
-    return few_rows(id_args(w, x, *v, nullptr), v->pairs, 16);
-}
-
 hipError_t mx4_product_float(const mx4_mat & w, int xtype, const void * x, int64_t ldx, int64_t x_rows, const moe_view * v,
                              int ytype, void * y, hipStream_t st) {
-    const mx4_mat xm = {nullptr, nullptr, x_rows, w.K};
+    const mx4_args a = product_args(w, {nullptr, nullptr, x_rows, w.K}, v, y);
     return with_type(xtype, [&](auto t) {
         using X = decltype(t);
-        if (v) return run_mv<1, X, true>(id_args(w, xm, *v, y), (const X *) x, ldx, ytype, st);
-        return run_mv<1, X, false>(product_args(w, xm, y), (const X *) x, ldx, ytype, st);
+        return v ? run_mv<1, X, true>(a, (const X *) x, ldx, ytype, st) : run_mv<1, X, false>(a, (const X *) x, ldx, ytype, st);
     });
 }
 

@@ -110,7 +110,8 @@ static __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tile(mx4_args a, un
     }
     const int64_t m0 = (int64_t) tm * S::TM;
     if (tr.n <= 0) return;
-    Y * y = (Y *) a.y;
+    // with K in shares, each writes sums of its own
+    Y * y = (Y *) a.y + (int64_t) blockIdx.y * a.T * a.M;
     if (IDS && tr.expert < 0) {   // pairs that no expert takes
         const int64_t cols = min((int64_t) S::TM, a.M - m0);
         for (int64_t i = threadIdx.x; i < S::TM * tr.n; i += 64 * S::NW)
@@ -142,13 +143,14 @@ static __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tile(mx4_args a, un
     const unsigned lds0 = (unsigned) (uintptr_t) (lds_char *) lds;
     // the block that this lane copies: its rows are 8 (wave + k NW) + lane / 8, NW even
     const int blk = (lane & 7) ^ ((wave & 1) * 4 + (lane >> 4));
-    const int last = (a.KB + 7) / 8 - 1;
+    const int planes = (a.KB + 7) / 8, share = (planes + gridDim.y - 1) / gridDim.y, first = blockIdx.y * share;
+    const int last = min(share, planes - first) - 1;   // this workgroup's planes, from `first` on
     // copy c of plane h into its place in the ring; past the last plane that one comes again, into a
     // place that nothing reads any more, so that the number of copies on their way is always known
     auto copy = [&](int h, auto cc) {
         constexpr int c = cc;
         const unsigned to = lds0 + h % STAGES * S::STAGE;
-        const int p = min(h, last);
+        const int p = first + min(h, last);
         if constexpr (c < CK) dma16(code_row[c] + (int64_t) min(p * 8 + blk, a.KB - 1) * 16, to + (wave + c * S::NW) * 1024);
         else dma4(exp_row[c - CK] + p * exp_step[c - CK], to + S::CODES + (wave + (c - CK) * S::NW) * 256);
     };
@@ -168,7 +170,7 @@ static __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tile(mx4_args a, un
         for (int i = 0; i < FN; ++i) nb[i] = *(const int *) (eb + at + i * 32 * 8);
     };
     auto take_exps = [&](int h) {   // this lane's four blocks', 0 past K
-        const int left = min(max(a.KB - h * 8 - 4 * half, 0), 4);
+        const int left = min(max(a.KB - (first + h) * 8 - 4 * half, 0), 4);
         const int mask = left == 4 ? ~0 : (1 << (8 * left)) - 1;
 #pragma unroll
         for (int i = 0; i < FM; ++i) sa[i] = na[i] & mask;
@@ -277,14 +279,47 @@ static __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tile(mx4_args a, un
     }
 }
 
+// y = the shares' sums, one after the other
+template <class Y> static __global__ void __launch_bounds__(256) k_mx4_join(const float * __restrict__ part, int64_t n, int shares, Y * __restrict__ y) {
+    const int64_t i = ((int64_t) blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= n) return;
+    if (i + 4 <= n) {
+        float s[4] = {};
+#pragma unroll 4
+        for (int k = 0; k < shares; ++k) {
+            const pack<float, 4> v = get<float, 4>(part + k * n + i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[j] += v.v[j];
+        }
+        for (int j = 0; j < 4; ++j) y[i + j] = from_f32<Y>(s[j]);
+    } else {
+        for (int64_t j = i; j < n; ++j) {
+            float s = 0.0f;
+            for (int k = 0; k < shares; ++k) s += part[k * n + j];
+            y[j] = from_f32<Y>(s);
+        }
+    }
+}
+
 template <int FM, int FN, int WM, int WN, int STAGES, bool IDS>
-static hipError_t run_tile(const mx4_args & a, int ytype, hipStream_t st) {
+static hipError_t run_tile(const mx4_args & a, int shares, float * part, int ytype, hipStream_t st) {
     using S = tile_shape<FM, FN, WM, WN, STAGES>;
     const int64_t tm = (a.M + S::TM - 1) / S::TM, tn = IDS ? id_tiles(a, S::TN) : (a.T + S::TN - 1) / S::TN;
     if (tm * tn > MAX_WAVES / S::NW) return hipErrorInvalidConfiguration;
+    const dim3 grid((unsigned) (tm * tn), shares);
+    auto go = [&](auto t, const mx4_args & a) {
+        k_mx4_tile<FM, FN, WM, WN, STAGES, decltype(t), IDS><<<grid, 64 * S::NW, S::LDS, st>>>(a, (unsigned) tm, (unsigned) tn);
+        return hipGetLastError();
+    };
+    if (shares == 1) return with_type(ytype, [&](auto t) { return go(t, a); });
+    mx4_args to_part = a;
+    to_part.y = part;
+    const hipError_t e = go(float{}, to_part);
+    if (e != hipSuccess) return e;
+    const int64_t n = a.T * a.M;
     return with_type(ytype, [&](auto t) {
         using Y = decltype(t);
-        k_mx4_tile<FM, FN, WM, WN, STAGES, Y, IDS><<<(unsigned) (tm * tn), 64 * S::NW, S::LDS, st>>>(a, (unsigned) tm, (unsigned) tn);
+        k_mx4_join<Y><<<(unsigned) ((n + 1023) / 1024), 256, 0, st>>>(part, n, shares, (Y *) a.y);
         return hipGetLastError();
     });
 }
@@ -300,26 +335,56 @@ static hipError_t run_tile(const mx4_args & a, int ytype, hipStream_t st) {
 // Deep rings serve CUs that have one tile (512 x 4096 x 14336: 38 us with four planes, 58 with two),
 // shallow ones let several share a CU (2048 x 4096 x 4096: 27 and 24; experts' tiles of 64, 300 tokens
 // by 8 experts of 4096 x 4096: 24 and 20).
-template <bool IDS> static hipError_t pick_tile(const mx4_args & a, int ytype, hipStream_t st) {
+// A long K over few tiles is cut into shares whose sums a second kernel joins: 128 x 4096 x 14336 22 -> 18
+// us, 64 x 4096 x 14336 24 -> 14, 100 x 640 x 14336 21 -> 10.5.
+struct tile_choice {
+    int side, stages, shares;
+};
+
+static tile_choice pick_tile(const mx4_args & a, bool ids) {
     constexpr double CUS = 256;
-    const double planes = (a.KB + 7) / 8;
-    auto load = [&](int side) {   // tiles per CU
-        const int64_t busy = a.T < a.n_expert ? a.T : a.n_expert;
-        const double n = IDS ? (double) a.T / side + 0.25 * busy : (double) ((a.T + side - 1) / side);
-        return n * ((a.M + side - 1) / side) / CUS;
-    };
-    auto rounds = [](double n) { return IDS ? std::max(n + 0.5, 1.0) : std::ceil(n); };
-    const double n256 = load(256), n128 = load(128), n64 = load(64);
-    const double t256 = rounds(n256) * (planes * 2.1 + 8);
-    const double t128 = n128 <= 1 ? rounds(n128) * (planes * 0.65 + 4) : rounds(n128) * planes * 0.8 + rounds(n128 / 2) * 4;
-    const double t64 = n64 <= 1 ? rounds(n64) * (planes * 0.33 + 4) : rounds(n64) * planes * 0.26 + rounds(n64 / 4) * 4;
-    if (t256 <= t128 && t256 <= t64) return run_tile<4, 2, 2, 4, 2, IDS>(a, ytype, st);
-    if (t128 <= t64) return n128 <= 1 ? run_tile<2, 2, 2, 2, 4, IDS>(a, ytype, st) : run_tile<2, 2, 2, 2, 2, IDS>(a, ytype, st);
-    return run_tile<1, 2, 2, 1, IDS ? 2 : 4, IDS>(a, ytype, st);
+    const int planes = (a.KB + 7) / 8;
+    auto rounds = [&](double n) { return ids ? std::max(n + 0.5, 1.0) : std::ceil(n); };
+    tile_choice best = {};
+    double least = 0;
+    for (const int side : {256, 128, 64}) {
+        const int64_t busy = std::min(a.T, (int64_t) a.n_expert);
+        const double cols = ids ? (double) a.T / side + 0.25 * busy : (double) ((a.T + side - 1) / side);
+        const double tiles = cols * ((a.M + side - 1) / side) / CUS;   // for each CU
+        for (int shares = 1; shares <= 16 && (shares == 1 || planes >= 2 * shares); shares *= 2) {
+            const double n = tiles * shares, p = (planes + shares - 1) / shares;
+            double t;
+            if (side == 256) t = rounds(n) * (p * 2.1 + 8);
+            else if (side == 128) t = n <= 1 ? rounds(n) * (p * 0.65 + 4) : rounds(n) * p * 0.8 + rounds(n / 2) * 4;
+            else t = n <= 1 ? rounds(n) * (p * 0.33 + 4) : rounds(n) * p * 0.26 + rounds(n / 4) * 4;
+            // the join: a launch, and the sums written and read
+            if (shares > 1) t += 3 + (double) shares * a.T * a.M * 8 / 4e6;
+            if (least == 0 || t < least) {
+                least = t;
+                best = {side, side == 256 ? 2 : side == 128 ? (n <= 1 ? 4 : 2) : (ids ? 2 : 4), shares};
+            }
+        }
+    }
+    // every share has planes of its own
+    while (best.shares > 1 && (planes + best.shares - 1) / best.shares * (best.shares - 1) >= planes) best.shares /= 2;
+    return best;
 }
 
-hipError_t mx4_product_tile(const mx4_args & a, int ytype, hipStream_t st) {
-    return a.offsets ? pick_tile<true>(a, ytype, st) : pick_tile<false>(a, ytype, st);
+int64_t mx4_tile_workspace(const mx4_args & a) {
+    const tile_choice c = pick_tile(a, a.n_expert != 0);
+    return c.shares > 1 ? c.shares * a.T * a.M * (int64_t) sizeof(float) : 0;
+}
+
+template <bool IDS> static hipError_t product_tile(const mx4_args & a, float * part, int ytype, hipStream_t st) {
+    const tile_choice c = pick_tile(a, IDS);
+    if (c.side == 256) return run_tile<4, 2, 2, 4, 2, IDS>(a, c.shares, part, ytype, st);
+    if (c.side == 128 && c.stages == 4) return run_tile<2, 2, 2, 2, 4, IDS>(a, c.shares, part, ytype, st);
+    if (c.side == 128) return run_tile<2, 2, 2, 2, 2, IDS>(a, c.shares, part, ytype, st);
+    return run_tile<1, 2, 2, 1, IDS ? 2 : 4, IDS>(a, c.shares, part, ytype, st);
+}
+
+hipError_t mx4_product_tile(const mx4_args & a, float * part, int ytype, hipStream_t st) {
+    return a.n_expert ? product_tile<true>(a, part, ytype, st) : product_tile<false>(a, part, ytype, st);
 }
 
 }  // namespace mi355x_ops

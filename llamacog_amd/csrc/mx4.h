@@ -102,7 +102,9 @@ struct mx4_args {
     void * y;
 };
 
-hipError_t mx4_product_tile(const mx4_args & a, int ytype, hipStream_t st);   // k_mx4_gemm.hip; by experts with a.offsets
+// k_mx4_gemm.hip; by experts where a.n_expert is not 0.  part: mx4_tile_workspace(a) bytes
+int64_t mx4_tile_workspace(const mx4_args & a);
+hipError_t mx4_product_tile(const mx4_args & a, float * part, int ytype, hipStream_t st);
 
 // waves of a launch: its threads are counted in 32 bits
 constexpr int64_t MAX_WAVES = ((int64_t) 1 << 32) / 64 - 1;

@@ -150,7 +150,8 @@ SIGNATURES = {
     "mi355x_moe_combine": [I, P, L, L, L, L, P, P, P, P],
     "mi355x_moe_combine_back": [I, P, L, P, L, L, L, L, P, P, P, P, P, P],
     "mi355x_mx4_scales_bytes": [L, L],
-    "mi355x_mx4_mul_mat_workspace": [L, L],
+    "mi355x_mx4_mul_mat_workspace": [L, L, I, L],
+    "mi355x_mx4_mul_mat_id_workspace": [L, L, L, I, L, L, I],
     "mi355x_moe_sort_workspace": [L, L, L],
 }
 
@@ -187,7 +188,8 @@ REFUSED = [
     ("mi355x_mx4_mul_mat_id", (A, A, 8, 64, 0, 0, A, None, 64, 3, 2, 0, A, A, 0, A, A, 1 << 20), -2),
     ("mi355x_mx4_mul_mat_id", (A, A, 8, 64, 1025, 0, A, None, 64, 3, 2, 0, A, A, 0, A, A, 1 << 20), -2),
     ("mi355x_mx4_mul_mat_id", (A, A, 8, 64, 4, 0, A, None, 64, 3, 17, 0, A, A, 0, A, A, 1 << 20), -2),
-    ("mi355x_mx4_mul_mat_id", (A, A, 8, 64, 4, 0, A, None, 64, 3, 2, 1, A, A, 0, A, A, 303), -4),
+    ("mi355x_mx4_mul_mat", (A, A, 640, 14336, -4, A, A, 0, 100, 0, A, A, 100 * 640 * 4), -4),
+    ("mi355x_mx4_mul_mat_id", (A, A, 8, 64, 4, 0, A, None, 64, 30, 2, 1, A, A, 0, A, A, 2000), -4),
     ("mi355x_moe_sort", (A, 4, 3, 0, 4, A, A, A, None, 0), -2),
     ("mi355x_moe_sort", (A, 4, 1 << 30, 2, 4, A, A, A, None, 0), -2),
     ("mi355x_moe_sort", (A, 2, 3, 2, 4, A, A, A, None, 0), -1),
@@ -228,7 +230,14 @@ def test_flat_calls_with_nothing_to_do(name, args):
 def test_sizes():
     scales, work, sort = flat("mi355x_mx4_scales_bytes"), flat("mi355x_mx4_mul_mat_workspace"), flat("mi355x_moe_sort_workspace")
     assert scales(3, 288) == 2 * 3 * 8 and scales(3, 289) == -1
-    assert work(3, 288) == 512 + 48 and work(3, 0) == -1
+    assert work(8, 0, 0, 3) == -1 and work(8, 288, 7, 3) == -1 and work(8, 288, 0, 0) == 0
+    assert work(8, 288, 0, 1) == 0                      # quantised where it is used
+    assert work(8, 288, 0, 3) == 512 + 256 and work(8, 288, -4, 3) == 0
+    assert work(640, 14336, -4, 100) % (100 * 640 * 4) == 0 and work(640, 14336, -4, 100) > 0   # sums of shares of K
+    shares = [work(m, k, -4, t) // (m * t * 4) for t, m, k in ((33, 48, 8192), (129, 70, 4128), (100, 17, 2592))]
+    assert shares == [16, 4, 0]
+    ids = flat("mi355x_mx4_mul_mat_id_workspace")
+    assert ids(8, 288, 4, 0, 100, 2, 0) > 0 and ids(8, 288, 0, 0, 100, 2, 0) == -1 and ids(8, 288, 4, 0, 100, 17, 0) == -1
     assert sort(10, 2, 8) == 0 and sort(1, 17, 8) == -1 and sort(1 << 20, 2, 8) > 0
 
 
@@ -319,6 +328,34 @@ def test_product(t, m, k, dtype):
     # quantised by the caller, and to another type
     assert torch.equal(ops.mx4_mul_mat(w, ops.mx4_quantize(x), dtype), y)
     check_product(ops.mx4_mul_mat(w, x, torch.float32), w64, np_rounded(x64), torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("t,m,k", [(33, 48, 8192), (40, 70, 8224), (129, 70, 4128), (64, 300, 14336), (100, 17, 2592), (257, 64, 5120)])
+def test_product_in_shares_of_k(t, m, k):
+    """Few tiles and a long K: sums of shares joined by a second kernel, a last share that is shorter, and
+    a K that is just not cut (test_sizes says which are)."""
+    rng = np.random.default_rng(t)
+    w, w64 = random_mx4(rng, m, k)
+    x, x64 = rows_of(rng, t, k, torch.bfloat16)
+    for dtype in TYPES:
+        check_product(ops.mx4_mul_mat(w, x, dtype), w64, np_rounded(x64), dtype)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["even", "holes", "one", "none"])
+def test_experts_product_in_shares_of_k(kind):
+    assert flat("mi355x_mx4_mul_mat_id_workspace")(33, 8224, 2, -4, 90, 2, 0) > 0
+    rng = np.random.default_rng(9)
+    ids, order, rank, plan = plan_of(rng, 90, 2, 2, kind)
+    held = int((order >= 0).sum())
+    w, w64 = random_mx4(rng, 2, 33, 8224)
+    x, x64 = rows_of(rng, 90, 8224, torch.float16)
+    y = ops.mx4_mul_mat_id(w, x, plan)
+    assert (y[held:] == 0).all()
+    for e in range(2):
+        at = np.flatnonzero(ids.reshape(-1)[order[:held]] == e)
+        check_product(y[torch.from_numpy(at).cuda()], w64[e], np_rounded(x64)[order[at] // 2], torch.float16)
 
 
 @gpu
