@@ -10,6 +10,7 @@ import ctypes
 import os
 import re
 import subprocess
+import threading
 
 import numpy as np
 import pytest
@@ -624,6 +625,78 @@ def test_streams_and_repeatability():
             got.append([expert_layer(*args) for _ in range(5)])
     torch.cuda.synchronize()
     assert all(torch.equal(want, y) for ys in got for y in ys)
+
+
+@gpu
+def test_two_threads_at_once():
+    """Calls from two threads, each on its own stream, give what one call gives."""
+    args, _ = layer_case(33)
+    want = expert_layer(*args)
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            ys = [expert_layer(*args) for _ in range(20)]
+            torch.cuda.current_stream().synchronize()
+            got[i] = all(torch.equal(want, y) for y in ys)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert got == [True, True]
+
+
+@gpu
+def test_offsets_past_32_bits_in_weights():
+    """Codes of 4.6 GB: the last rows of a long matrix and of the last of many experts."""
+    m, k = 1_100_000, 8384
+    codes = torch.randint(0, 256, (m, k // 2), dtype=torch.uint8, device="cuda")
+    scales = torch.randint(120, 130, (-(-k // 256), m, 8), dtype=torch.uint8, device="cuda")
+    assert codes.numel() > 1 << 32
+    w, end = ops.Mx4(codes, scales), ops.Mx4(codes[-100:].clone(), scales[:, -100:].contiguous())
+    for t in (1, 20, 40):
+        x = torch.randn(t, k, device="cuda")
+        y, want = ops.mx4_mul_mat(w, x), ops.mx4_mul_mat(end, x)
+        assert torch.allclose(y[:, -100:], want, rtol=1e-5, atol=float(want.abs().max()) * 1e-5)   # other kernels, other sums
+    del w
+    n_expert, rows = 1000, 1100
+    stack = ops.Mx4(codes.view(n_expert, rows, k // 2), scales.view(n_expert, -(-k // 256), rows, 8))
+    ids = torch.tensor([[999, 0], [5, 999], [999, 998]], device="cuda")
+    x = torch.randn(3, k, device="cuda")
+    plan = ops.moe_sort(ids, n_expert)
+    y = ops.mx4_mul_mat_id(stack, x, plan)
+    for t, j in ((0, 0), (1, 1), (2, 0), (2, 1)):
+        e = int(ids[t, j])
+        want = ops.mx4_mul_mat(ops.Mx4(stack.codes[e], stack.scales[e]), x[t:t + 1])
+        assert torch.allclose(y[int(plan.rank[t, j])], want[0], rtol=1e-5, atol=float(want.abs().max()) * 1e-5)
+
+
+@gpu
+def test_offsets_past_32_bits_in_rows():
+    """2.3 G elements of sorted rows: gathered, combined and back, looked at from the far end."""
+    t, used, d = 70_000, 8, 4096
+    ids = torch.randint(0, 16, (t, used), dtype=torch.int32, device="cuda")
+    plan = ops.moe_sort(ids, 16)
+    x = torch.randint(-8, 9, (t, d), device="cuda").to(torch.bfloat16)
+    xs = ops.moe_gather(x, plan)
+    assert xs.numel() > 1 << 31
+    order = plan.order.long()
+    for at in (0, t * used - 1000):
+        assert torch.equal(xs[at:at + 1000], x[order[at:at + 1000] // used])
+    w = torch.randint(-2, 3, (t, used), device="cuda").float()     # small whole numbers: every sum is exact
+    y = ops.moe_combine(xs, plan, w)
+    assert torch.equal(y[-500:].float(), (x[-500:].float() * w[-500:].sum(1, keepdim=True)).to(torch.bfloat16).float())
+    dys, dw = ops.moe_combine_back(x, xs, plan, w)
+    assert torch.equal(dw[-500:], (x[-500:].float() ** 2).sum(1, keepdim=True).expand(-1, used))
+    at = t * used - 1000
+    assert torch.equal(dys[at:], x[order[at:] // used] * w.flatten()[order[at:], None].to(torch.bfloat16))
+    q = ops.mx4_quantize(xs)
+    end = ops.mx4_quantize(xs[-100:])
+    assert torch.equal(q.codes[-100:], end.codes) and torch.equal(q.scales[:, -100:], end.scales)
+    assert torch.equal(ops.mx4_dequantize(q, torch.bfloat16)[-100:], ops.mx4_dequantize(end, torch.bfloat16))
 
 
 @gpu
