@@ -270,7 +270,8 @@ static __global__ void __launch_bounds__(256) k_moe_combine(row_args a, const T 
 
 // Each slot's row read and its gradient written; a token's lanes (up to a workgroup) go through its
 // columns and join their dot products, in a wave by exchanges, over waves in shared memory, always
-// in the same order.
+// in the same order.  A token's slots follow one another, so that its dy row comes from memory once;
+// where the tokens are too few to fill the card, every slot has lanes of its own (gridDim.y).
 template <class T, bool WHOLE, bool STREAM>
 static __global__ void __launch_bounds__(256) k_moe_combine_back(row_args a, const T * __restrict__ dy, int64_t lddy,
                                                                  const T * __restrict__ ys, int64_t ldys,
@@ -283,7 +284,7 @@ static __global__ void __launch_bounds__(256) k_moe_combine_back(row_args a, con
     const int lanes = 1 << a.lsh, mine = threadIdx.x & (lanes - 1);
     const int64_t t = (int64_t) blockIdx.x * (256 >> a.lsh) + (threadIdx.x >> a.lsh);
     const bool here = t < a.T;
-    for (int j = 0; j < a.used; ++j) {
+    for (int j = blockIdx.y; j < a.used; j += gridDim.y) {
         float dot = 0.0f;
         if (here) {
             const int64_t p = t * a.used + j, r = rank[p];
@@ -313,7 +314,7 @@ static __global__ void __launch_bounds__(256) k_moe_combine_back(row_args a, con
     }
     if (lanes <= 64) return;
     __syncthreads();
-    if (here && mine < a.used) {
+    if (here && mine < a.used && mine % gridDim.y == blockIdx.y) {
         const int wave = threadIdx.x >> 6;
         float s = part[wave][mine] + part[wave + 1][mine];
         if (lanes == 256) s += part[2][mine] + part[3][mine];
@@ -357,9 +358,13 @@ hipError_t moe_combine_back(int type, const void * dy, int64_t lddy, const void 
                             int used, const int32_t * order, const int32_t * rank, const float * w, void * dys, float * dw,
                             hipStream_t st) {
     const bool stream = T * used * D * (type == ELEM_F32 ? 4 : 2) > STREAM_BYTES;
-    return with_rows(type, T, D, used, stream, [&](auto t, auto whole, auto flag, const row_args & a, dim3 grid) {
+    return with_rows(type, T, D, used, stream, [&](auto t, auto whole, auto flag, row_args a, dim3) {
         using E = decltype(t);
-        k_moe_combine_back<E, whole, flag><<<grid.x, 256, 0, st>>>(a, (const E *) dy, lddy, (const E *) ys, ldys, order, rank, w,
+        // here a lane may have several columns: no more lanes than columns, so that none is idle for long
+        if (a.lsh > 0 && ((int64_t) COLS<E> << a.lsh) > D + COLS<E> - 1) --a.lsh;
+        dim3 groups(ceil_div(T, 256 >> a.lsh));
+        groups.y = groups.x < 2048 ? used : 1;
+        k_moe_combine_back<E, whole, flag><<<groups, 256, 0, st>>>(a, (const E *) dy, lddy, (const E *) ys, ldys, order, rank, w,
                                                                    (E *) dys, dw);
         return hipGetLastError();
     });
