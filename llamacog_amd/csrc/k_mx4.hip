@@ -192,7 +192,7 @@ static __global__ void __launch_bounds__(64 * MV_WAVES, 4) k_mx4_mv(mx4_args a, 
     const uint8_t * xl[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) xl[n] = lds + min(16 * n + r, (int) tr.n - 1) * row_bytes;
-    float * red = (float *) (lds + min((int64_t) 16 * NT, a.T) * row_bytes);   // [GW][KS][16 NT][16]
+    float * red = (float *) (lds + min((int64_t) 16 * NT, a.T) * row_bytes);   // [GW][KS][16][16]
 
     for (int64_t g = g0; g * 16 < a.M; g += (int64_t) per_tile * GW) {
         v4f acc[NT] = {};
@@ -225,18 +225,20 @@ static __global__ void __launch_bounds__(64 * MV_WAVES, 4) k_mx4_mv(mx4_args a, 
                     for (int i = 0; i < 4; ++i)
                         if (m0 + 4 * q + i < a.M) y[(16 * n + r) * a.M + m0 + 4 * q + i] = from_f32<Y>(acc[n][i]);
         } else {
-            __syncthreads();   // the sums of the groups before have been taken
 #pragma unroll
-            for (int n = 0; n < NT; ++n) *(v4f *) &red[((wave * NT + n) * 16 + r) * 16 + 4 * q] = acc[n];
-            __syncthreads();
-            for (int i = threadIdx.x; i < GW * NT * 256; i += 64 * MV_WAVES) {
-                const int k = i / (NT * 256), t = i / 16 % (16 * NT);
-                const int64_t m = (g + k) * 16 + i % 16;
-                if (t >= tr.n || m >= a.M) continue;
-                float sum = 0.0f;
+            for (int n = 0; n < NT; ++n) {   // 16 x rows at a time, to leave shared memory for another workgroup
+                __syncthreads();             // the sums before have been taken
+                *(v4f *) &red[(wave * 16 + r) * 16 + 4 * q] = acc[n];
+                __syncthreads();
+                for (int i = threadIdx.x; i < GW * 256; i += 64 * MV_WAVES) {
+                    const int k = i / 256, t = 16 * n + i / 16 % 16;
+                    const int64_t m = (g + k) * 16 + i % 16;
+                    if (t >= tr.n || m >= a.M) continue;
+                    float sum = 0.0f;
 #pragma unroll
-                for (int p = 0; p < KS; ++p) sum += red[(k * KS + p) * NT * 256 + i % (NT * 256)];
-                y[t * a.M + m] = from_f32<Y>(sum);
+                    for (int p = 0; p < KS; ++p) sum += red[(k * KS + p) * 256 + i % 256];
+                    y[t * a.M + m] = from_f32<Y>(sum);
+                }
             }
         }
     }
@@ -245,7 +247,7 @@ static __global__ void __launch_bounds__(64 * MV_WAVES, 4) k_mx4_mv(mx4_args a, 
 constexpr int64_t MV_LDS = 144 * 1024;   // most shared memory of a workgroup
 
 static int64_t mv_lds(const mx4_args & a, int NT, int KS) {
-    return mv_row_bytes(a.KB) * (a.T < 16 * NT ? a.T : 16 * NT) + (KS > 1 ? MV_WAVES * NT * 1024 : 0);
+    return mv_row_bytes(a.KB) * (a.T < 16 * NT ? a.T : 16 * NT) + (KS > 1 ? MV_WAVES * 1024 : 0);
 }
 
 // how many waves share a group of 16 weight rows: as few as give `tiles` tiles MV_FILL waves in all
