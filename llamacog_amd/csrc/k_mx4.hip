@@ -16,26 +16,25 @@ static inline unsigned ceil_div(int64_t a, int64_t b) { return (unsigned) ((a + 
 // Bound by memory: 2 or 4 B read and 17/32 B written per element.  A lane takes 8 elements (a
 // 16-B load of the 16-bit types), four lanes a block: their maximum is two DPP steps, and the
 // conversion is the hardware's (v_cvt_scalef32_pk_fp4: one rounding, saturating).  Lanes are laid
-// over a row's columns in a power of two so that no division is needed; a workgroup takes R times
-// as many rows as its lanes hold, loads first: QROWS to keep bytes in flight, one where that leaves
-// fewer than QFEW workgroups (29 x 4096: 4.8 us with four, 2.3 with one).
-constexpr int QROWS = 4, QFEW = 1024;
+// over a row's columns in a power of two so that no division is needed; a workgroup takes QROWS
+// times as many rows as its lanes hold, loads first, to keep bytes in flight.
+constexpr int QROWS = 4;
 
-template <class T, int R>
+template <class T>
 static __global__ void __launch_bounds__(256) k_mx4_quantize(const T * __restrict__ x, int64_t ldx, int64_t rows, int64_t K, int lsh,
                                                       uint8_t * __restrict__ codes, uint8_t * __restrict__ scales) {
     const int64_t c = (int64_t) blockIdx.y << lsh | (threadIdx.x & ((1 << lsh) - 1));
     if (c >= K / 8) return;   // K / 8 is a multiple of four: the four lanes of a block stay together
     const int rp = 256 >> lsh;
-    const int64_t row0 = (int64_t) blockIdx.x * rp * R + (threadIdx.x >> lsh);
-    float v[R][8];
+    const int64_t row0 = (int64_t) blockIdx.x * rp * QROWS + (threadIdx.x >> lsh);
+    float v[QROWS][8];
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
+    for (int i = 0; i < QROWS; ++i) {
         const int64_t row = min(row0 + (int64_t) i * rp, rows - 1);
         load8(x + row * ldx + c * 8, v[i]);
     }
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
+    for (int i = 0; i < QROWS; ++i) {
         const int64_t row = row0 + (int64_t) i * rp;
         if (row >= rows) break;
         const unsigned e = mx4_block_exponent(v[i]);
@@ -59,13 +58,10 @@ static int row_shift(int64_t cols) {   // log2 of the lanes laid over a row of `
 hipError_t mx4_quantize(int type, const void * x, int64_t ldx, int64_t rows, int64_t K, uint8_t * codes, uint8_t * scales,
                         hipStream_t st) {
     const int lsh = row_shift(K / 8);
-    const int64_t per = 256 >> lsh, cols = ceil_div(K / 8, 1 << lsh);
-    const bool few = (rows + per * QROWS - 1) / (per * QROWS) * cols < QFEW;
-    const dim3 grid(ceil_div(rows, few ? per : per * QROWS), cols);
+    const dim3 grid(ceil_div(rows, (int64_t) (256 >> lsh) * QROWS), ceil_div(K / 8, 1 << lsh));
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        auto * k = few ? k_mx4_quantize<T, 1> : k_mx4_quantize<T, QROWS>;
-        k<<<grid, 256, 0, st>>>((const T *) x, ldx, rows, K, lsh, codes, scales);
+        k_mx4_quantize<T><<<grid, 256, 0, st>>>((const T *) x, ldx, rows, K, lsh, codes, scales);
         return hipGetLastError();
     });
 }
