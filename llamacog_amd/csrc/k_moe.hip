@@ -21,7 +21,9 @@ static inline unsigned ceil_div(int64_t a, int64_t b) { return (unsigned) ((a + 
 // find each other by one ballot per bit of the id, the lowest of them keeps the wave's count.
 // One chunk is one launch; more are two: the chunks' counts, then their places, where every
 // workgroup sums the counts in front of its own (at most SORT_CHUNKS of them).  Bound by latency:
-// ids are loaded SORT_LOADS at a time, the chunks' counts are summed by all threads.
+// ids are loaded SORT_LOADS at a time, the chunks' counts are summed by all threads.  2 pairs 3.2 us,
+// 4000 5.8, 131072 by 128 experts 15 (both launches).  Chunks of 8192 and 16384 took longer: 4000 pairs
+// 8.3 and 13.3 us a call instead of 6.4, 16000 11.5 and 16.8 instead of 11.5.
 constexpr int SORT_WAVES = 16;
 constexpr int SORT_LOADS = 4;
 constexpr int SORT_CHUNK = SORT_WAVES * SORT_LOADS * 64;    // least pairs of a chunk
@@ -194,7 +196,9 @@ hipError_t moe_sort(const void * ids, int id_bytes, int64_t pairs, int n_expert,
 // All three are bound by memory: every row is read once and written once, a token's row once for
 // all of its slots (the gather goes by rank, not by order, for that).  A lane owns 16 bytes of a
 // token's columns, the last one what is left; lanes are laid over the columns in a power of two.
-// Rows lie on any address.
+// Rows lie on any address.  16384 tokens, 8 slots, 2048 bf16 columns: gather 102 us (5.9 TB/s, nearly all
+// writes, past the caches: 112 through them), combine 127 (4.7 TB/s), back 228 (5.0 TB/s); with 2047
+// columns 142, 137 and 307.
 struct row_args {
     int64_t T, D, pairs;
     int used, lsh;   // slots; log2 of the lanes over a row

@@ -14,6 +14,10 @@
 //     that belongs in its slot.
 //   - Past K both exponents are 0, so that the product of two codes vanishes (2^-254 of it).
 //   - Past M and T rows repeat the last one; their results are not stored.
+// Bound by power: on random codes the card holds this kernel at 1.6 - 1.7 GHz (2.2 on zeros, where it takes
+// 0.71 of the time), as it does the instruction alone (6.15 PFLOP/s).  2048 x 28672 x 8192 255 us, 3.8
+// PFLOP/s; 4096 x 4096 x 28672 247 us, 3.9 PFLOP/s.  A row's 128 B of a plane are a whole cache line: planes of
+// half that, in a ring of four, took 9 % longer.
 #include "mx4.h"
 
 #include <algorithm>
