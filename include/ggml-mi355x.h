@@ -141,9 +141,9 @@ double mi355x_bench_op(int which, int64_t a, int64_t b, int iters);
 #define MI355X_STREAM_DEFAULT ((void *) 1)
 #define MI355X_MX4 (-4)             // an operand given as MXFP4 codes and scales
 #define MI355X_ERR_TYPE (-1)
-#define MI355X_ERR_SHAPE (-2)
+#define MI355X_ERR_SHAPE (-2)        // a size that is not supported, or NULL where there is something to do
 #define MI355X_ERR_ALIGN (-3)       // codes and workspaces 16 bytes, scales 8, the rest its element
-#define MI355X_ERR_WORKSPACE (-4)
+#define MI355X_ERR_WORKSPACE (-4)    // smaller than the workspace call says
 #define MI355X_ERR_HIP (-5)
 
 // MXFP4 rows: codes [rows][K / 2], element 2 i in the low half of byte i, E2M1 (sign, then 0 0.5 1

@@ -39,6 +39,9 @@ bool is_elem(int t) { return t == ELEM_F32 || t == ELEM_F16 || t == ELEM_BF16; }
 int64_t elem_size(int t) { return t == ELEM_F32 ? 4 : 2; }
 bool aligned(const void * p, uintptr_t n) { return (uintptr_t) p % n == 0; }
 
+// where there is something to do, a pointer that the call needs is not NULL
+template <class... P> int present(const P *... p) { return ((p != nullptr) && ...) ? 0 : MI355X_ERR_SHAPE; }
+
 constexpr int64_t MAX_K = (int64_t) 1 << 24;       // elements of a row
 constexpr int64_t MAX_ROWS = (int64_t) 1 << 31;    // rows of a matrix, pairs of a routing step (exclusive)
 
@@ -83,6 +86,7 @@ OPS_API int mi355x_mx4_quantize(int xtype, const void * x, int64_t ldx, int64_t 
     TRY(check_mx4(codes, scales));
     if (ldx < K && rows > 1) return MI355X_ERR_SHAPE;
     if (rows == 0) return 0;
+    TRY(present(x, codes, scales));
     call_stream cs(stream);
     if (cs.err != hipSuccess) return MI355X_ERR_HIP;
     return cs.done(mx4_quantize(xtype, x, ldx, rows, K, codes, scales, cs.st));
@@ -94,6 +98,7 @@ OPS_API int mi355x_mx4_dequantize(const uint8_t * codes, const uint8_t * scales,
     TRY(check_elems(ytype, y));
     TRY(check_mx4(codes, scales));
     if (rows == 0) return 0;
+    TRY(present(codes, scales, y));
     call_stream cs(stream);
     if (cs.err != hipSuccess) return MI355X_ERR_HIP;
     return cs.done(mx4_dequantize({codes, scales, rows, K}, ytype, y, cs.st));
@@ -132,7 +137,11 @@ struct product {
         TRY(check_elems(ytype, y));
         if (!aligned(work, 16)) return MI355X_ERR_ALIGN;
         if (x_rows == 0 || w.rows == 0) return 0;
-        if (work_bytes < workspace()) return MI355X_ERR_WORKSPACE;
+        TRY(present(w.codes, w.scales, x, y));
+        if (xtype == MI355X_MX4) TRY(present(x_scales));
+        if (view) TRY(present(view->order, view->offsets));
+        const int64_t needed = workspace();
+        if (work_bytes < needed || (needed && !work)) return MI355X_ERR_WORKSPACE;
         call_stream cs(stream);
         if (cs.err != hipSuccess) return MI355X_ERR_HIP;
         if (xtype == MI355X_MX4)
@@ -190,7 +199,10 @@ OPS_API int mi355x_moe_sort(const void * ids, int id_bytes, int64_t T, int64_t u
     if (n_expert <= 0 || n_expert > MOE_MAX_EXPERTS) return MI355X_ERR_SHAPE;
     if (id_bytes != 4 && id_bytes != 8) return MI355X_ERR_TYPE;
     if (!aligned(ids, id_bytes) || !aligned(work, 4)) return MI355X_ERR_ALIGN;
-    if (work_bytes < (int64_t) moe_sort_workspace(T * used, (int) n_expert)) return MI355X_ERR_WORKSPACE;
+    TRY(present(offsets));
+    if (T > 0) TRY(present(ids, order, rank));
+    const int64_t needed = (int64_t) moe_sort_workspace(T * used, (int) n_expert);
+    if (work_bytes < needed || (needed && !work)) return MI355X_ERR_WORKSPACE;
     call_stream cs(stream);
     if (cs.err != hipSuccess) return MI355X_ERR_HIP;
     return cs.done(moe_sort(ids, id_bytes, T * used, (int) n_expert, order, rank, offsets, work, cs.st));
@@ -203,6 +215,7 @@ OPS_API int mi355x_moe_gather(int type, const void * x, int64_t ldx, int64_t T, 
     TRY(check_elems(type, xs));
     if (D < 0 || D > MAX_K || (ldx < D && T > 1)) return MI355X_ERR_SHAPE;
     if (T == 0 || D == 0) return 0;
+    TRY(present(x, order, rank, xs));
     call_stream cs(stream);
     if (cs.err != hipSuccess) return MI355X_ERR_HIP;
     return cs.done(moe_gather(type, x, ldx, T, D, (int) used, order, rank, xs, cs.st));
@@ -215,6 +228,7 @@ OPS_API int mi355x_moe_combine(int type, const void * ys, int64_t ldys, int64_t 
     TRY(check_elems(type, y));
     if (D < 0 || D > MAX_K || (ldys < D && T * used > 1)) return MI355X_ERR_SHAPE;
     if (T == 0 || D == 0) return 0;
+    TRY(present(ys, rank, y));   // w may be NULL
     call_stream cs(stream);
     if (cs.err != hipSuccess) return MI355X_ERR_HIP;
     return cs.done(moe_combine(type, ys, ldys, T, D, (int) used, rank, w, y, cs.st));
@@ -228,8 +242,9 @@ OPS_API int mi355x_moe_combine_back(int type, const void * dy, int64_t lddy, con
     TRY(check_elems(type, ys));
     TRY(check_elems(type, dys));
     if (D < 0 || D > MAX_K || (lddy < D && T > 1) || (ldys < D && T * used > 1)) return MI355X_ERR_SHAPE;
-    if (!w) return MI355X_ERR_SHAPE;
     if (T == 0) return 0;
+    TRY(present(order, rank, w, dw));
+    if (D > 0) TRY(present(dy, ys, dys));
     call_stream cs(stream);
     if (cs.err != hipSuccess) return MI355X_ERR_HIP;
     return cs.done(moe_combine_back(type, dy, lddy, ys, ldys, T, D, (int) used, order, rank, w, dys, dw, cs.st));

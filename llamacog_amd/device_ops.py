@@ -38,6 +38,14 @@ if not os.path.exists(BINDING):
     raise BackendMissing(f"operators not built: {BINDING} is missing (run __graft_entry__.build())")
 from . import _device_ops as _ops  # noqa: E402
 
+# torch brings a HIP runtime of its own.  The plugin, loaded later, uses that one too; loaded before, it
+# has brought the system's, and two runtimes in a process do not know of each other's work.
+with open("/proc/self/maps") as _maps:
+    _runtimes = {line.split()[-1] for line in _maps if "libamdhip64" in line}
+if len(_runtimes) > 1:
+    raise ImportError("two HIP runtimes in this process: import llamacog_amd.device_ops (or torch) before the plugin is loaded: "
+                      + ", ".join(sorted(_runtimes)))
+
 
 class Mx4(NamedTuple):
     """MXFP4 rows.  codes uint8 [..., rows, K / 2]: element 2 i in the low half of byte i, E2M1.

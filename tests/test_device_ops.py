@@ -206,6 +206,21 @@ REFUSED = [
 ]
 
 
+N = None
+REFUSED += [(n, a, -2) for n, a in [
+    ("mi355x_mx4_quantize", (0, N, 64, 3, 64, A, A)), ("mi355x_mx4_quantize", (0, A, 64, 3, 64, N, A)),
+    ("mi355x_mx4_quantize", (0, A, 64, 3, 64, A, N)), ("mi355x_mx4_dequantize", (A, N, 3, 64, 0, A)),
+    ("mi355x_mx4_dequantize", (A, A, 3, 64, 0, N)), ("mi355x_mx4_mul_mat", (N, A, 8, 64, 0, A, N, 64, 3, 0, A, A, 1 << 20)),
+    ("mi355x_mx4_mul_mat", (A, A, 8, 64, -4, A, N, 64, 3, 0, A, A, 1 << 20)), ("mi355x_mx4_mul_mat", (A, A, 8, 64, 0, A, N, 64, 3, 0, N, A, 1 << 20)),
+    ("mi355x_mx4_mul_mat_id", (A, A, 8, 64, 4, 0, A, N, 64, 3, 2, 0, N, A, 0, A, A, 1 << 20)),
+    ("mi355x_mx4_mul_mat_id", (A, A, 8, 64, 4, 0, A, N, 64, 3, 2, 0, A, N, 0, A, A, 1 << 20)),
+    ("mi355x_moe_sort", (N, 4, 3, 2, 4, A, A, A, N, 0)), ("mi355x_moe_sort", (A, 4, 3, 2, 4, A, A, N, N, 0)), ("mi355x_moe_sort", (N, 4, 0, 2, 4, N, N, N, N, 0)),
+    ("mi355x_moe_gather", (0, A, 9, 3, 9, 2, N, A, A)), ("mi355x_moe_combine", (0, A, 9, 3, 9, 2, N, A, A)),
+    ("mi355x_moe_combine_back", (0, A, 9, A, 9, 3, 9, 2, A, A, A, A, N)),
+]]
+REFUSED += [("mi355x_mx4_mul_mat", (A, A, 8, 64, 0, A, N, 64, 3, 0, A, N, 1 << 20), -4), ("mi355x_moe_sort", (A, 4, 1 << 20, 2, 4, A, A, A, N, 1 << 30), -4)]
+
+
 @pytest.mark.parametrize("name,args,code", REFUSED, ids=[f"{n[7:]}-{i}" for i, (n, _, _) in enumerate(REFUSED)])
 def test_flat_calls_refused_before_any_launch(name, args, code):
     assert flat(name)(*args, None) == code
