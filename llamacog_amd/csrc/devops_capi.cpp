@@ -61,8 +61,11 @@ int check_elems(int type, const void * p) {
     return aligned(p, (uintptr_t) elem_size(type)) ? 0 : MI355X_ERR_ALIGN;
 }
 
+// integers and float32 weights, in as many arrays as the call has
+template <class... P> int check_words(const P *... p) { return (aligned(p, 4) && ...) ? 0 : MI355X_ERR_ALIGN; }
+
 int check_routing(int64_t T, int64_t used) {
-    if (T < 0 || used <= 0 || used > MOE_MAX_USED || T * used >= MAX_ROWS) return MI355X_ERR_SHAPE;
+    if (used <= 0 || used > MOE_MAX_USED || T < 0 || T >= MAX_ROWS || T * used >= MAX_ROWS) return MI355X_ERR_SHAPE;
     return 0;
 }
 
@@ -135,6 +138,7 @@ struct product {
         else TRY(check_elems(xtype, x));
         if (xtype != MI355X_MX4 && ldx < w.K && x_rows > 1) return MI355X_ERR_SHAPE;
         TRY(check_elems(ytype, y));
+        if (view) TRY(check_words(view->order, view->offsets));
         if (!aligned(work, 16)) return MI355X_ERR_ALIGN;
         if (x_rows == 0 || w.rows == 0) return 0;
         TRY(present(w.codes, w.scales, x, y));
@@ -199,6 +203,7 @@ OPS_API int mi355x_moe_sort(const void * ids, int id_bytes, int64_t T, int64_t u
     if (n_expert <= 0 || n_expert > MOE_MAX_EXPERTS) return MI355X_ERR_SHAPE;
     if (id_bytes != 4 && id_bytes != 8) return MI355X_ERR_TYPE;
     if (!aligned(ids, id_bytes) || !aligned(work, 4)) return MI355X_ERR_ALIGN;
+    TRY(check_words(order, rank, offsets));
     TRY(present(offsets));
     if (T > 0) TRY(present(ids, order, rank));
     const int64_t needed = (int64_t) moe_sort_workspace(T * used, (int) n_expert);
@@ -213,6 +218,7 @@ OPS_API int mi355x_moe_gather(int type, const void * x, int64_t ldx, int64_t T, 
     TRY(check_routing(T, used));
     TRY(check_elems(type, x));
     TRY(check_elems(type, xs));
+    TRY(check_words(order, rank));
     if (D < 0 || D > MAX_K || (ldx < D && T > 1)) return MI355X_ERR_SHAPE;
     if (T == 0 || D == 0) return 0;
     TRY(present(x, order, rank, xs));
@@ -226,6 +232,7 @@ OPS_API int mi355x_moe_combine(int type, const void * ys, int64_t ldys, int64_t 
     TRY(check_routing(T, used));
     TRY(check_elems(type, ys));
     TRY(check_elems(type, y));
+    TRY(check_words(rank, w));
     if (D < 0 || D > MAX_K || (ldys < D && T * used > 1)) return MI355X_ERR_SHAPE;
     if (T == 0 || D == 0) return 0;
     TRY(present(ys, rank, y));   // w may be NULL
@@ -241,6 +248,7 @@ OPS_API int mi355x_moe_combine_back(int type, const void * dy, int64_t lddy, con
     TRY(check_elems(type, dy));
     TRY(check_elems(type, ys));
     TRY(check_elems(type, dys));
+    TRY(check_words(order, rank, w, dw));
     if (D < 0 || D > MAX_K || (lddy < D && T > 1) || (ldys < D && T * used > 1)) return MI355X_ERR_SHAPE;
     if (T == 0) return 0;
     TRY(present(order, rank, w, dw));

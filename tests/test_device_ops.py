@@ -220,6 +220,25 @@ REFUSED += [(n, a, -2) for n, a in [
 ]]
 REFUSED += [("mi355x_mx4_mul_mat", (A, A, 8, 64, 0, A, N, 64, 3, 0, A, N, 1 << 20), -4), ("mi355x_moe_sort", (A, 4, 1 << 20, 2, 4, A, A, A, N, 1 << 30), -4)]
 
+# sizes whose product passes 64 bits
+REFUSED += [(n, a, -2) for n, a in [
+    ("mi355x_moe_sort", (A, 4, 1 << 62, 4, 4, A, A, A, N, 0)), ("mi355x_moe_gather", (0, A, 9, 1 << 62, 9, 4, A, A, A)),
+    ("mi355x_moe_combine", (0, A, 9, 1 << 60, 9, 16, A, A, A)), ("mi355x_moe_combine_back", (0, A, 9, A, 9, 1 << 61, 9, 8, A, A, A, A, A)),
+    ("mi355x_mx4_mul_mat_id", (A, A, 8, 64, 4, 0, A, N, 64, 1 << 62, 4, 1, A, A, 0, A, A, 1 << 20)),
+    ("mi355x_moe_gather", (0, A, 9, 3, 9, (1 << 62) + 2, A, A, A)),
+]]
+# integers and weights that lie between elements
+REFUSED += [(n, a, -3) for n, a in [
+    ("mi355x_moe_sort", (A, 4, 3, 2, 4, A + 2, A, A, N, 0)), ("mi355x_moe_sort", (A, 4, 3, 2, 4, A, A + 1, A, N, 0)),
+    ("mi355x_moe_sort", (A, 4, 3, 2, 4, A, A, A + 2, N, 0)), ("mi355x_moe_gather", (0, A, 9, 3, 9, 2, A + 2, A, A)),
+    ("mi355x_moe_gather", (0, A, 9, 3, 9, 2, A, A + 2, A)), ("mi355x_moe_combine", (1, A, 9, 3, 9, 2, A + 2, A, A)),
+    ("mi355x_moe_combine", (1, A, 9, 3, 9, 2, A, A + 2, A)), ("mi355x_moe_combine_back", (1, A, 9, A, 9, 3, 9, 2, A + 2, A, A, A, A)),
+    ("mi355x_moe_combine_back", (1, A, 9, A, 9, 3, 9, 2, A, A + 2, A, A, A)), ("mi355x_moe_combine_back", (1, A, 9, A, 9, 3, 9, 2, A, A, A + 2, A, A)),
+    ("mi355x_moe_combine_back", (1, A, 9, A, 9, 3, 9, 2, A, A, A, A, A + 2)),
+    ("mi355x_mx4_mul_mat_id", (A, A, 8, 64, 4, 0, A, N, 64, 3, 2, 0, A + 2, A, 0, A, A, 1 << 20)),
+    ("mi355x_mx4_mul_mat_id", (A, A, 8, 64, 4, 0, A, N, 64, 3, 2, 0, A, A + 2, 0, A, A, 1 << 20)),
+]]
+
 
 @pytest.mark.parametrize("name,args,code", REFUSED, ids=[f"{n[7:]}-{i}" for i, (n, _, _) in enumerate(REFUSED)])
 def test_flat_calls_refused_before_any_launch(name, args, code):
