@@ -42,10 +42,16 @@ void no_gradient(const Tensor & t, const char * what) {
                       ": no gradient is recorded here; pass a detached tensor");
 }
 
+// its memory holds the values: not a view that negates them
+void plain(const Tensor & t, const char * what) {
+    TORCH_CHECK_VALUE(t.layout() == at::kStrided && !t.is_neg(), what, ": a strided tensor that is no lazily negated view is wanted");
+}
+
 // a float [rows, columns] tensor whose columns lie side by side and whose rows do not overlap; returns its type
 int matrix(const Tensor & t, const char * what) {
     on_gpu(t, what);
     const int type = elem_type(t.scalar_type(), what);
+    plain(t, what);
     TORCH_CHECK_VALUE(t.dim() == 2, what, ": [rows, columns] is wanted, got ", t.sizes());
     TORCH_CHECK_VALUE((t.stride(1) == 1 || t.size(1) <= 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1)), what,
                       ": columns have to lie side by side and rows apart, got strides ", t.strides());
@@ -58,6 +64,7 @@ int64_t row_step(const Tensor & t) { return t.size(0) > 1 ? t.stride(0) : t.size
 
 void whole(const Tensor & t, const char * what, const Tensor & other, at::ScalarType type, at::IntArrayRef shape) {
     beside(t, what, other);
+    plain(t, what);
     TORCH_CHECK_TYPE(t.scalar_type() == type, what, ": ", type, " is wanted, got ", t.scalar_type());
     TORCH_CHECK_VALUE(t.sizes() == shape && t.is_contiguous(), what, ": a contiguous tensor of shape ", shape,
                       " is wanted, got ", t.sizes(), ", strides ", t.strides());
@@ -73,6 +80,7 @@ struct mx4 {
 
 mx4 check_mx4(const Tensor & codes, const Tensor & scales, const char * what, int dims) {
     on_gpu(codes, what);
+    plain(codes, what);
     TORCH_CHECK_TYPE(codes.scalar_type() == at::kByte, what, ".codes: uint8 is wanted, got ", codes.scalar_type());
     TORCH_CHECK_VALUE(codes.dim() == dims && codes.is_contiguous(), what, ".codes: a contiguous tensor of ", dims,
                       " dimensions is wanted, got ", codes.sizes(), ", strides ", codes.strides());
@@ -224,6 +232,7 @@ Tensor mul_mat_id(const Tensor & w_codes, const Tensor & w_scales, const Tensor 
 
 std::tuple<Tensor, Tensor, Tensor> sort(const Tensor & ids, int64_t n_expert) {
     on_gpu(ids, "ids");
+    plain(ids, "ids");
     TORCH_CHECK_TYPE(ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong, "ids: int32 or int64 is wanted, got ",
                      ids.scalar_type());
     TORCH_CHECK_VALUE(ids.dim() == 2 && ids.is_contiguous(), "ids: a contiguous [T, used] tensor is wanted, got ", ids.sizes(),

@@ -208,7 +208,7 @@ template <class T> constexpr int COLS = 16 / sizeof(T);
 
 static __device__ __forceinline__ bool my_columns(const row_args & a, int N, int64_t & t, int64_t & col) {
     col = ((int64_t) blockIdx.y << a.lsh | (threadIdx.x & ((1 << a.lsh) - 1))) * N;
-    t = (int64_t) blockIdx.x * (256 >> a.lsh) + (threadIdx.x >> a.lsh);
+    t = row_group() * (256 >> a.lsh) + (threadIdx.x >> a.lsh);
     return t < a.T && col < a.D;
 }
 
@@ -286,7 +286,7 @@ static __global__ void __launch_bounds__(256) k_moe_combine_back(row_args a, con
     constexpr int N = COLS<T>;
     __shared__ float part[4][MOE_MAX_USED];
     const int lanes = 1 << a.lsh, mine = threadIdx.x & (lanes - 1);
-    const int64_t t = (int64_t) blockIdx.x * (256 >> a.lsh) + (threadIdx.x >> a.lsh);
+    const int64_t t = row_group() * (256 >> a.lsh) + (threadIdx.x >> a.lsh);
     const bool here = t < a.T;
     for (int j = blockIdx.y; j < a.used; j += gridDim.y) {
         float dot = 0.0f;
@@ -333,7 +333,7 @@ template <class F> static hipError_t with_rows(int type, int64_t T, int64_t D, i
         row_args a{T, D, T * used, used, 0};
         const int64_t cols = (D + COLS<E> - 1) / COLS<E>;
         while (a.lsh < 8 && (1 << a.lsh) < cols) ++a.lsh;
-        const dim3 grid(ceil_div(T, 256 >> a.lsh), ceil_div(cols, (int64_t) 1 << a.lsh));
+        const dim3 grid = row_groups(ceil_div(T, 256 >> a.lsh), ceil_div(cols, (int64_t) 1 << a.lsh));
         auto with_flag = [&](auto whole) { return flag ? f(t, whole, std::true_type{}, a, grid) : f(t, whole, std::false_type{}, a, grid); };
         return D % COLS<E> == 0 ? with_flag(std::true_type{}) : with_flag(std::false_type{});
     });
@@ -366,8 +366,8 @@ hipError_t moe_combine_back(int type, const void * dy, int64_t lddy, const void 
         using E = decltype(t);
         // here a lane may have several columns: no more lanes than columns, so that none is idle for long
         if (a.lsh > 0 && ((int64_t) COLS<E> << a.lsh) > D + COLS<E> - 1) --a.lsh;
-        dim3 groups(ceil_div(T, 256 >> a.lsh));
-        groups.y = groups.x < 2048 ? used : 1;
+        const int64_t n = ceil_div(T, 256 >> a.lsh);
+        const dim3 groups = row_groups(n, n < 2048 ? used : 1);
         k_moe_combine_back<E, whole, flag><<<groups, 256, 0, st>>>(a, (const E *) dy, lddy, (const E *) ys, ldys, order, rank, w,
                                                                    (E *) dys, dw);
         return hipGetLastError();

@@ -27,7 +27,7 @@ static __global__ void __launch_bounds__(256) k_mx4_quantize(const T * __restric
     const int64_t c = (int64_t) blockIdx.y << lsh | (threadIdx.x & ((1 << lsh) - 1));
     if (c >= K / 8) return;   // K / 8 is a multiple of four: the four lanes of a block stay together
     const int rp = 256 >> lsh;
-    const int64_t row0 = (int64_t) blockIdx.x * rp * QROWS + (threadIdx.x >> lsh);
+    const int64_t row0 = row_group() * rp * QROWS + (threadIdx.x >> lsh);
     float v[QROWS][8];
 #pragma unroll
     for (int i = 0; i < QROWS; ++i) {
@@ -59,7 +59,7 @@ static int row_shift(int64_t cols) {   // log2 of the lanes laid over a row of `
 hipError_t mx4_quantize(int type, const void * x, int64_t ldx, int64_t rows, int64_t K, uint8_t * codes, uint8_t * scales,
                         hipStream_t st) {
     const int lsh = row_shift(K / 8);
-    const dim3 grid(ceil_div(rows, (int64_t) (256 >> lsh) * QROWS), ceil_div(K / 8, 1 << lsh));
+    const dim3 grid = row_groups(ceil_div(rows, (int64_t) (256 >> lsh) * QROWS), ceil_div(K / 8, 1 << lsh));
     return with_type(type, [&](auto t) {
         using T = decltype(t);
         k_mx4_quantize<T><<<grid, 256, 0, st>>>((const T *) x, ldx, rows, K, lsh, codes, scales);
@@ -75,7 +75,7 @@ static __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t * _
     const int64_t c = (int64_t) blockIdx.y << lsh | (threadIdx.x & ((1 << lsh) - 1));
     if (c >= K / 8) return;
     const int rp = 256 >> lsh;
-    const int64_t row0 = (int64_t) blockIdx.x * rp * QROWS + (threadIdx.x >> lsh);
+    const int64_t row0 = row_group() * rp * QROWS + (threadIdx.x >> lsh);
     uint32_t q[QROWS];
     unsigned e[QROWS];
 #pragma unroll
@@ -96,7 +96,7 @@ static __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t * _
 
 hipError_t mx4_dequantize(const mx4_mat & m, int type, void * y, hipStream_t st) {
     const int lsh = row_shift(m.K / 8);
-    const dim3 grid(ceil_div(m.rows, (int64_t) (256 >> lsh) * QROWS), ceil_div(m.K / 8, 1 << lsh));
+    const dim3 grid = row_groups(ceil_div(m.rows, (int64_t) (256 >> lsh) * QROWS), ceil_div(m.K / 8, 1 << lsh));
     return with_type(type, [&](auto t) {
         using T = decltype(t);
         k_mx4_dequantize<T><<<grid, 256, 0, st>>>(m.codes, m.scales, m.rows, m.K, lsh, (T *) y);

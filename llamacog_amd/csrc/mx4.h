@@ -106,9 +106,6 @@ struct mx4_args {
 int64_t mx4_tile_workspace(const mx4_args & a);
 hipError_t mx4_product_tile(const mx4_args & a, float * part, int ytype, hipStream_t st);
 
-// waves of a launch: its threads are counted in 32 bits
-constexpr int64_t MAX_WAVES = ((int64_t) 1 << 32) / 64 - 1;
-
 // bytes of an x row in shared memory: codes and exponents, an odd number of 16-B columns, so that the
 // same column of 16 rows lies in 16 different ones of the banks
 __host__ __device__ constexpr int mv_row_bytes(int KB) { return (KB + (KB + 15) / 16 | 1) * 16; }

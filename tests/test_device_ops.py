@@ -733,6 +733,71 @@ def test_offsets_past_32_bits_in_rows():
     assert torch.equal(ops.mx4_dequantize(q, torch.bfloat16)[-100:], ops.mx4_dequantize(end, torch.bfloat16))
 
 
+def far_rows(t, d, dtype):
+    """[t, d] whose rows differ: 1024 random ones over and over, the row's number in the first three columns."""
+    torch.cuda.empty_cache()
+    x = torch.empty(t, d, dtype=dtype, device="cuda")
+    some = torch.randn(1024, d, device="cuda").to(dtype)
+    whole = t // 1024 * 1024
+    x[:whole].view(-1, 1024, d)[:] = some
+    x[whole:] = some[:t - whole]
+    n = torch.arange(t, device="cuda")
+    for c in range(3):
+        x[:, c] = (n >> 8 * c & 255).to(dtype)
+    return x
+
+
+def enough_memory(bytes):
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < bytes:
+        pytest.skip(f"{bytes >> 30} GiB of the card's memory are wanted")
+
+
+@gpu
+def test_rows_past_32_bits_of_threads():
+    """More tokens than one axis of a launch has workgroups of 256, each with one token's row."""
+    t, d = (1 << 24) + 77, 2048
+    enough_memory(215 << 30)
+    x = far_rows(t, d, torch.bfloat16)
+    plan = ops.moe_sort(torch.randint(-1, 3, (t, 1), dtype=torch.int32, device="cuda"), 3)
+    rank = plan.rank.view(-1).long()
+    xs = ops.moe_gather(x, plan)
+    parts = [slice(i, i + (1 << 18)) for i in range(0, t, 1 << 18)]
+    for s in parts:
+        held = rank[s] >= 0
+        assert torch.equal(xs[rank[s][held]], x[s][held])
+    assert not xs[int(plan.offsets[-1]):].any()
+    weights = torch.full((t, 1), 0.5, device="cuda")
+    y = ops.moe_combine(xs, plan, weights)
+    for s in parts:
+        assert torch.equal(y[s], torch.where(rank[s][:, None] >= 0, x[s] * 0.5, 0.0))
+    del y
+    dys, dw = ops.moe_combine_back(x, xs, plan, weights)
+    for s in parts:
+        assert torch.equal(dys[s], xs[s] * 0.5)
+        want = torch.where(rank[s] >= 0, (x[s].float() ** 2).sum(1), 0.0)
+        # two float32 sums of 2048 squares
+        assert torch.allclose(dw[s, 0], want, rtol=2 * 2048 * half_step(torch.float32), atol=0)
+
+
+@gpu
+def test_quantize_past_32_bits_of_threads():
+    """As many workgroups, four rows in each."""
+    t, d = (1 << 26) + 77, 1056
+    enough_memory(215 << 30)
+    x = far_rows(t, d, torch.bfloat16)
+    m = ops.mx4_quantize(x)
+    parts = [slice(i, i + (1 << 20)) for i in range(0, t, 1 << 20)]
+    for s in parts:
+        want = ops.mx4_quantize(x[s])
+        assert torch.equal(m.codes[s], want.codes) and torch.equal(m.scales[:, s], want.scales)
+    del x
+    torch.cuda.empty_cache()
+    y = ops.mx4_dequantize(m, torch.bfloat16)
+    for s in parts:
+        assert torch.equal(y[s], ops.mx4_dequantize(ops.Mx4(m.codes[s], m.scales[:, s].contiguous()), torch.bfloat16))
+
+
 @gpu
 def test_flat_abi_on_a_private_stream():
     """stream NULL: done when the call returns."""
@@ -776,6 +841,11 @@ def test_tensors_refused_on_the_host():
         (TypeError, lambda: ops.moe_combine_back(x.half(), rows, plan, weights)), (ValueError, lambda: ops.moe_combine_back(x[:3], rows, plan, weights)),
         (ValueError, lambda: ops.moe_combine_back(x, rows, plan, weights.clone().requires_grad_())),
     ]
+    bad += [(ValueError, call) for call in [
+        lambda: ops.mx4_quantize(torch._neg_view(x)), lambda: ops.mx4_quantize(x.to_sparse()), lambda: ops.mx4_mul_mat(w, torch._neg_view(x)),
+        lambda: ops.moe_combine(rows, plan, torch._neg_view(weights)), lambda: ops.moe_sort(torch._neg_view(plan.rank), 3),
+        lambda: ops.moe_combine_back(torch._neg_view(x), rows, plan, weights),
+    ]]
     for i, (kind, call) in enumerate(bad):
         with pytest.raises(kind):
             call()
