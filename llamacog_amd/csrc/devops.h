@@ -10,6 +10,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <tuple>
 #include <type_traits>
 
 namespace mi355x_ops {
@@ -71,6 +72,21 @@ constexpr int64_t MAX_WAVES = ((int64_t) 1 << 32) / 64 - 1;
 static inline dim3 row_groups(int64_t n, int64_t y) {
     const int64_t z = (n + MAX_WAVES / 4 - 1) / (MAX_WAVES / 4);
     return dim3((unsigned) ((n + z - 1) / z), (unsigned) y, (unsigned) z);
+}
+
+// A launch and its own status.  hipGetLastError would also name an earlier failure, of any HIP call that the
+// thread made, and take it from whoever has yet to ask; it is asked only to clear what this launch left.
+template <class... P, class... A>
+static inline hipError_t launch(void (*kernel)(P...), dim3 grid, unsigned threads, size_t lds, hipStream_t st, A... args) {
+    std::tuple<P...> values(args...);
+    return std::apply(
+        [&](auto &... v) {
+            void * at[] = {(void *) &v...};
+            const hipError_t e = hipLaunchKernel((const void *) kernel, grid, dim3(threads), at, lds, st);
+            if (e != hipSuccess) (void) hipGetLastError();
+            return e;
+        },
+        values);
 }
 
 // ---- device side -----------------------------------------------------------------------------

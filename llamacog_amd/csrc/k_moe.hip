@@ -182,12 +182,12 @@ hipError_t moe_sort(const void * ids, int id_bytes, int64_t pairs, int n_expert,
     const size_t lds = (size_t) SORT_WAVES * n_expert * sizeof(int);
     auto go = [&](auto i) {
         using I = decltype(i);
-        if (n > 1)
-            k_moe_sort<I, true><<<n, 64 * SORT_WAVES, lds, st>>>((const I *) ids, pairs, chunk, n_expert, bits,
-                                                                 (int32_t *) work, order, rank, offsets);
-        k_moe_sort<I, false><<<n, 64 * SORT_WAVES, lds, st>>>((const I *) ids, pairs, chunk, n_expert, bits, (int32_t *) work,
-                                                              order, rank, offsets);
-        return hipGetLastError();
+        auto pass = [&](auto kernel) {
+            return launch(kernel, n, 64 * SORT_WAVES, lds, st, (const I *) ids, pairs, chunk, n_expert, bits, (int32_t *) work, order, rank,
+                          offsets);
+        };
+        const hipError_t e = n > 1 ? pass(k_moe_sort<I, true>) : hipSuccess;
+        return e == hipSuccess ? pass(k_moe_sort<I, false>) : e;
     };
     return id_bytes == 8 ? go(int64_t{}) : go(int32_t{});
 }
@@ -344,8 +344,7 @@ hipError_t moe_gather(int type, const void * x, int64_t ldx, int64_t T, int64_t 
     const bool stream = T * used * D * (type == ELEM_F32 ? 4 : 2) > STREAM_BYTES;
     return with_rows(type, T, D, used, stream, [&](auto t, auto whole, auto flag, const row_args & a, dim3 grid) {
         using E = decltype(t);
-        k_moe_gather<E, whole, flag><<<grid, 256, 0, st>>>(a, (const E *) x, ldx, order, rank, (E *) xs);
-        return hipGetLastError();
+        return launch(k_moe_gather<E, whole, flag>, grid, 256, 0, st, a, (const E *) x, ldx, order, rank, (E *) xs);
     });
 }
 
@@ -353,8 +352,7 @@ hipError_t moe_combine(int type, const void * ys, int64_t ldys, int64_t T, int64
                        const float * w, void * y, hipStream_t st) {
     return with_rows(type, T, D, used, w != nullptr, [&](auto t, auto whole, auto flag, const row_args & a, dim3 grid) {
         using E = decltype(t);
-        k_moe_combine<E, whole, flag><<<grid, 256, 0, st>>>(a, (const E *) ys, ldys, rank, w, (E *) y);
-        return hipGetLastError();
+        return launch(k_moe_combine<E, whole, flag>, grid, 256, 0, st, a, (const E *) ys, ldys, rank, w, (E *) y);
     });
 }
 
@@ -368,9 +366,8 @@ hipError_t moe_combine_back(int type, const void * dy, int64_t lddy, const void 
         if (a.lsh > 0 && ((int64_t) COLS<E> << a.lsh) > D + COLS<E> - 1) --a.lsh;
         const int64_t n = ceil_div(T, 256 >> a.lsh);
         const dim3 groups = row_groups(n, n < 2048 ? used : 1);
-        k_moe_combine_back<E, whole, flag><<<groups, 256, 0, st>>>(a, (const E *) dy, lddy, (const E *) ys, ldys, order, rank, w,
-                                                                   (E *) dys, dw);
-        return hipGetLastError();
+        return launch(k_moe_combine_back<E, whole, flag>, groups, 256, 0, st, a, (const E *) dy, lddy, (const E *) ys, ldys, order, rank, w,
+                      (E *) dys, dw);
     });
 }
 

@@ -62,8 +62,7 @@ hipError_t mx4_quantize(int type, const void * x, int64_t ldx, int64_t rows, int
     const dim3 grid = row_groups(ceil_div(rows, (int64_t) (256 >> lsh) * QROWS), ceil_div(K / 8, 1 << lsh));
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        k_mx4_quantize<T><<<grid, 256, 0, st>>>((const T *) x, ldx, rows, K, lsh, codes, scales);
-        return hipGetLastError();
+        return launch(k_mx4_quantize<T>, grid, 256, 0, st, (const T *) x, ldx, rows, K, lsh, codes, scales);
     });
 }
 
@@ -99,8 +98,7 @@ hipError_t mx4_dequantize(const mx4_mat & m, int type, void * y, hipStream_t st)
     const dim3 grid = row_groups(ceil_div(m.rows, (int64_t) (256 >> lsh) * QROWS), ceil_div(m.K / 8, 1 << lsh));
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        k_mx4_dequantize<T><<<grid, 256, 0, st>>>(m.codes, m.scales, m.rows, m.K, lsh, (T *) y);
-        return hipGetLastError();
+        return launch(k_mx4_dequantize<T>, grid, 256, 0, st, m.codes, m.scales, m.rows, m.K, lsh, (T *) y);
     });
 }
 
@@ -275,8 +273,8 @@ static hipError_t run_mv(const mx4_args & a, const X * x, int64_t ldx, int ytype
             const int64_t fair = (768 + busy - 1) / busy;   // three workgroups per CU in all, each with its turn of the groups
             const int per_tile = (int) (rounds < fair ? rounds : fair);
             if (per_tile * tiles > MAX_WAVES / MV_WAVES) return hipErrorInvalidConfiguration;
-            k_mx4_mv<NT, KS, X, Y, IDS><<<(unsigned) (per_tile * tiles), 64 * MV_WAVES, mv_lds(a, NT, KS), st>>>(a, x, ldx, per_tile);
-            return hipGetLastError();
+            return launch(k_mx4_mv<NT, KS, X, Y, IDS>, (unsigned) (per_tile * tiles), 64 * MV_WAVES, mv_lds(a, NT, KS), st, a, x, ldx,
+                          per_tile);
         };
         switch (ks) {
             case 1: return go(std::integral_constant<int, 1>{});

@@ -312,8 +312,7 @@ static hipError_t run_tile(const mx4_args & a, int shares, float * part, int yty
     if (tm * tn > MAX_WAVES / S::NW) return hipErrorInvalidConfiguration;
     const dim3 grid((unsigned) (tm * tn), shares);
     auto go = [&](auto t, const mx4_args & a) {
-        k_mx4_tile<FM, FN, WM, WN, STAGES, decltype(t), IDS><<<grid, 64 * S::NW, S::LDS, st>>>(a, (unsigned) tm, (unsigned) tn);
-        return hipGetLastError();
+        return launch(k_mx4_tile<FM, FN, WM, WN, STAGES, decltype(t), IDS>, grid, 64 * S::NW, S::LDS, st, a, (unsigned) tm, (unsigned) tn);
     };
     if (shares == 1) return with_type(ytype, [&](auto t) { return go(t, a); });
     mx4_args to_part = a;
@@ -323,8 +322,7 @@ static hipError_t run_tile(const mx4_args & a, int shares, float * part, int yty
     const int64_t n = a.T * a.M;
     return with_type(ytype, [&](auto t) {
         using Y = decltype(t);
-        k_mx4_join<Y><<<(unsigned) ((n + 1023) / 1024), 256, 0, st>>>(part, n, shares, (Y *) a.y);
-        return hipGetLastError();
+        return launch(k_mx4_join<Y>, (unsigned) ((n + 1023) / 1024), 256, 0, st, part, n, shares, (Y *) a.y);
     });
 }
 

@@ -852,3 +852,39 @@ def test_tensors_refused_on_the_host():
             pytest.fail(f"call {i} was not refused")
     with torch.no_grad():
         ops.mx4_quantize(x.clone().requires_grad_())
+
+
+def hip_runtime():
+    """The HIP runtime of this process."""
+    with open("/proc/self/maps") as maps:
+        return ctypes.CDLL(next(line.split()[-1] for line in maps if "libamdhip64" in line))
+
+
+@gpu
+def test_calls_after_an_earlier_failure_of_the_thread():
+    """A HIP call that failed before, elsewhere in the program, neither fails a valid call nor is taken from
+    the one who has yet to ask for it."""
+    args, _ = layer_case(4)
+    x, ids, weights, up, _, n_expert = args
+    rng = np.random.default_rng(0)
+    w, _ = random_mx4(rng, 70, 4128)
+    many = torch.randn(129, 4128, device="cuda")          # tiles, K in shares
+    plan = ops.moe_sort(ids, n_expert)
+    wide = torch.randint(0, n_expert, (5000, 2), device="cuda")   # two launches
+    ys = torch.randn(8, 512, device="cuda")
+    calls = [lambda: ops.mx4_quantize(x), lambda: (ops.mx4_dequantize(up._replace(codes=up.codes[0], scales=up.scales[0])),),
+             lambda: (ops.mx4_mul_mat(w, many[:1]),), lambda: (ops.mx4_mul_mat(w, many),), lambda: (ops.mx4_mul_mat_id(up, x, plan),),
+             lambda: plan, lambda: ops.moe_sort(ids, n_expert), lambda: ops.moe_sort(wide, n_expert), lambda: (ops.moe_gather(x, plan),),
+             lambda: (ops.moe_combine(ys, plan, weights),), lambda: ops.moe_combine_back(x, ys, plan, weights)]
+    hip = hip_runtime()
+    for i, call in enumerate(calls):
+        want = call()
+        torch.cuda.synchronize()
+        failed = hip.hipSetDevice(-1)
+        assert failed != 0
+        try:
+            got = call()
+        finally:
+            left = hip.hipGetLastError()
+        assert left == failed, f"call {i}"
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), f"call {i}"
