@@ -3,6 +3,7 @@
 // smallest calls last a few microseconds on the device, less than argument handling takes in Python.
 // llamacog_amd/device_ops.py documents the functions; here are the checks, the output allocations
 // and the calls.
+#include <c10/core/AutogradState.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
@@ -37,9 +38,12 @@ void beside(const Tensor & t, const char * what, const Tensor & other) {
     TORCH_CHECK_VALUE(t.device() == other.device(), what, ": on ", t.device(), ", the others on ", other.device());
 }
 
+// neither a gradient is recorded nor a tangent passed on (forward mode, which no_grad() leaves on)
 void no_gradient(const Tensor & t, const char * what) {
     TORCH_CHECK_VALUE(!t.requires_grad() || !at::GradMode::is_enabled(), what,
                       ": no gradient is recorded here; pass a detached tensor");
+    TORCH_CHECK_VALUE(!t._fw_grad(0).defined() || !c10::AutogradState::get_tls_state().get_fw_grad_mode(), what,
+                      ": no tangent is passed on here; pass a tensor without one");
 }
 
 // its memory holds the values: not a view that negates them
@@ -49,13 +53,13 @@ void plain(const Tensor & t, const char * what) {
 
 // a float [rows, columns] tensor whose columns lie side by side and whose rows do not overlap; returns its type
 int matrix(const Tensor & t, const char * what) {
+    no_gradient(t, what);
     on_gpu(t, what);
     const int type = elem_type(t.scalar_type(), what);
     plain(t, what);
     TORCH_CHECK_VALUE(t.dim() == 2, what, ": [rows, columns] is wanted, got ", t.sizes());
     TORCH_CHECK_VALUE((t.stride(1) == 1 || t.size(1) <= 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1)), what,
                       ": columns have to lie side by side and rows apart, got strides ", t.strides());
-    no_gradient(t, what);
     return type;
 }
 
@@ -270,8 +274,8 @@ Tensor combine(const Tensor & ys, const Tensor & order, const Tensor & rank, con
     const plan p = check_plan(order, rank, offsets, ys);
     check_sorted(ys, p);
     if (weights) {
-        whole(*weights, "weights", ys, at::kFloat, {p.t, p.used});
         no_gradient(*weights, "weights");
+        whole(*weights, "weights", ys, at::kFloat, {p.t, p.used});
     }
     Tensor y = fresh({p.t, ys.size(1)}, ys, ys.scalar_type());
     launch on(ys);
@@ -290,8 +294,8 @@ std::tuple<Tensor, Tensor> combine_back(const Tensor & dy, const Tensor & ys, co
     matrix(dy, "dy");
     TORCH_CHECK_VALUE(dy.size(0) == p.t && dy.size(1) == ys.size(1), "dy: ", p.t, " rows of ", ys.size(1), " are wanted, got ", dy.sizes());
     TORCH_CHECK_TYPE(dy.scalar_type() == ys.scalar_type(), "dy: ", ys.scalar_type(), " is wanted, as ys has, got ", dy.scalar_type());
-    whole(weights, "weights", ys, at::kFloat, {p.t, p.used});
     no_gradient(weights, "weights");
+    whole(weights, "weights", ys, at::kFloat, {p.t, p.used});
     Tensor dys = fresh({p.t * p.used, ys.size(1)}, ys, ys.scalar_type()), dw = fresh({p.t, p.used}, ys, at::kFloat);
     launch on(ys);
     check(mi355x_moe_combine_back(type, dy.const_data_ptr(), row_step(dy), ys.const_data_ptr(), row_step(ys), p.t, ys.size(1), p.used,

@@ -5,8 +5,8 @@ Every function launches on torch's current stream of its tensors' device and ret
 waiting; nothing is kept between calls, and a call may be captured into a graph.  Arguments are
 checked on the host (ValueError, TypeError); what depends on values on the device is defined
 instead: expert ids outside 0 .. n_expert - 1 belong to no expert.  There is no CPU form, and no
-gradient is recorded: an input that asks for one is refused (moe_combine_back and, for moe_gather,
-moe_combine are the gradients).
+gradient is recorded: an input that asks for one, or carries a tangent of forward mode, is refused
+(moe_combine_back and, for moe_gather, moe_combine are the gradients).
 
     plan = moe_sort(ids, n_expert)                       # ids [T, used] from the router
     h = mx4_mul_mat_id(w_up, x, plan)                    # [T * used, F], rows sorted by expert

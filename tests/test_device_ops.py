@@ -888,3 +888,37 @@ def test_calls_after_an_earlier_failure_of_the_thread():
             left = hip.hipGetLastError()
         assert left == failed, f"call {i}"
         assert all(torch.equal(a, b) for a, b in zip(got, want)), f"call {i}"
+
+
+def tangent_calls(x, device):
+    """Calls with a tensor that carries a tangent: (call, does it get as far without a GPU)."""
+    dual = lambda *shape: torch.autograd.forward_ad.make_dual(torch.zeros(shape, device=device), torch.ones(shape, device=device))  # noqa: E731
+    tokens, rows, weights = (2, 64), (4, 64), (2, 2)
+    dual_x, dual_ys, dual_w = dual(*tokens), dual(*rows), dual(*weights)
+    ys, w = torch.zeros(rows, device=device), torch.zeros(weights, device=device)
+    plan = ops.MoePlan(torch.arange(4, dtype=torch.int32, device=device), torch.arange(4, dtype=torch.int32, device=device).view(2, 2),
+                       torch.tensor([0, 4], dtype=torch.int32, device=device))
+    m = ops.Mx4(torch.zeros(1, 3, 32, dtype=torch.uint8, device=device), torch.zeros(1, 1, 3, 8, dtype=torch.uint8, device=device))
+    return [
+        (lambda: ops.mx4_quantize(dual_x), True), (lambda: ops.moe_gather(dual_x, plan), True),
+        (lambda: ops.moe_combine(dual_ys, plan), True), (lambda: ops.moe_combine_back(x, dual_ys, plan, w), True),
+        (lambda: ops.mx4_mul_mat(ops.Mx4(m.codes[0], m.scales[0]), dual_x), False), (lambda: ops.mx4_mul_mat_id(m, dual_x, plan), False),
+        (lambda: ops.moe_combine(ys, plan, dual_w), False), (lambda: ops.moe_combine_back(dual_x, ys, plan, w), False),
+        (lambda: ops.moe_combine_back(x, ys, plan, dual_w), False),
+    ]
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_tangents_are_refused(device):
+    """Forward mode: a tangent would be dropped without a word.  no_grad() does not turn it off."""
+    with torch.autograd.forward_ad.dual_level():
+        for i, (call, anywhere) in enumerate(tangent_calls(torch.zeros(2, 64, device=device), device)):
+            if device == "cpu" and not anywhere:
+                continue
+            for mode in (torch.enable_grad(), torch.no_grad()):
+                with mode, pytest.raises(ValueError, match="tangent"):
+                    call()
+                    pytest.fail(f"call {i} was not refused")
+            if device == "cuda":
+                with torch.autograd.forward_ad._set_fwd_grad_enabled(False):
+                    call()
