@@ -922,3 +922,12 @@ def test_tangents_are_refused(device):
             if device == "cuda":
                 with torch.autograd.forward_ad._set_fwd_grad_enabled(False):
                     call()
+
+
+@pytest.mark.parametrize("target,binding", [("all", False), ("ops", False), ("torch", True)])
+def test_only_the_binding_is_built_against_torch(target, binding):
+    """What make would run for a target from nothing: the plugin and the flat library on a host without torch."""
+    csrc = os.path.join(la.PKG, "csrc")
+    out = subprocess.run(["make", "-n", "-B", "-C", csrc, target], capture_output=True, text=True, check=True).stdout
+    assert ("torch" in re.sub(r"make.*directory.*", "", out)) == binding
+    assert "libmi355x-ops.so" in out
