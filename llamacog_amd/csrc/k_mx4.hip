@@ -118,7 +118,6 @@ hipError_t mx4_dequantize(const mx4_mat & m, int type, void * y, hipStream_t st)
 //
 // One row: 4096 x 14336 9.5 us, 28672 x 4096 14.5 (4.3 TB/s), two experts of 28672 x 4096 25 (5.0 TB/s): about
 // 3 us until the first weights have come, then the memory's rate.
-constexpr int MV_WAVES = 8;
 
 // U planes of a row group
 template <int U> struct mv_weights {
@@ -243,28 +242,11 @@ static __global__ void __launch_bounds__(64 * MV_WAVES, 4) k_mx4_mv(mx4_args a, 
     }
 }
 
-constexpr int64_t MV_LDS = 144 * 1024;   // most shared memory of a workgroup, of a CU's 160 KiB
-
-static int64_t mv_lds(const mx4_args & a, int NT, int KS) {
-    return mv_row_bytes(a.KB) * (a.T < 16 * NT ? a.T : 16 * NT) + (KS > 1 ? MV_WAVES * 1024 : 0);
-}
-
-// how many waves share a group of 16 weight rows: as few as give `tiles` tiles MV_FILL waves in all.  With
-// 1024 / 2048 / 4096 / 8192, 4096 x 14336 by one row took 13.3 / 10.7 / 10.7 / 10.7 us, 32001 x 4096 by 29 rows
-// 21.1 / 21.1 / 22.2 / 21.5, 4096 x 14336 by 64 39 / 26 / 31 / 34.
-constexpr int64_t MV_FILL = 2048;
-static int mv_split(const mx4_args & a, int64_t tiles) {
-    const int64_t groups = (a.M + 15) / 16 * tiles;
-    int ks = 1;
-    while (ks < MV_WAVES && groups * ks < MV_FILL && a.KB > 8 * ks) ks *= 2;
-    return ks;
-}
-
 template <int NT, class X, bool IDS>
 static hipError_t run_mv(const mx4_args & a, const X * x, int64_t ldx, int ytype, hipStream_t st) {
     const int64_t tiles = IDS ? id_tiles(a, 16 * NT) : (a.T + 16 * NT - 1) / (16 * NT);
-    const int64_t busy = IDS ? (a.T < a.n_expert ? a.T : a.n_expert) : tiles;   // tiles to reckon with
-    const int ks = mv_split(a, busy);
+    const int64_t busy = mv_busy(a, NT);
+    const int ks = mv_split(a, NT);
     return with_type(ytype, [&](auto t) {
         using Y = decltype(t);
         auto go = [&](auto split) {
@@ -307,16 +289,6 @@ static mx4_args product_args(const mx4_mat & w, const mx4_mat & x, const moe_vie
     return a;
 }
 
-// The kernel for few rows, as long as its tiles of 16 or 32 rows read the weights about once: 4096 x
-// 4096 by 20 rows takes 5.6 us here and 9.2 in 64 x 64 tiles, 28672 x 4096 by 64 rows 28.6 and 18.5;
-// by experts up to 16 rows each.
-static bool few_rows(const mx4_args & a) {
-    return a.T <= (a.n_expert ? 16 * (int64_t) a.n_expert : 32) && mv_lds(a, 1, MV_WAVES) <= MV_LDS;
-}
-
-// few enough that every workgroup may quantise those of its tile
-static bool float_rows(const mx4_args & a) { return few_rows(a) && a.T <= (a.n_expert ? 16 : 2); }
-
 mx4_needs mx4_product_needs(const mx4_mat & w, int64_t x_rows, const moe_view * v) {
     const mx4_args a = product_args(w, {nullptr, nullptr, x_rows, w.K}, v, nullptr);
     return {!float_rows(a), few_rows(a) ? 0 : mx4_tile_workspace(a)};
@@ -327,8 +299,7 @@ hipError_t mx4_product(const mx4_mat & w, const mx4_mat & x, const moe_view * v,
     const mxfp4 * in = nullptr;
     if (!few_rows(a)) return mx4_product_tile(a, (float *) part, ytype, st);
     if (v) return run_mv<1, mxfp4, true>(a, in, 0, ytype, st);
-    if (a.T > 16 && mv_lds(a, 2, MV_WAVES) <= MV_LDS) return run_mv<2, mxfp4, false>(a, in, 0, ytype, st);
-    return run_mv<1, mxfp4, false>(a, in, 0, ytype, st);
+    return mv_tiles(a) == 2 ? run_mv<2, mxfp4, false>(a, in, 0, ytype, st) : run_mv<1, mxfp4, false>(a, in, 0, ytype, st);
 }
 
 hipError_t mx4_product_float(const mx4_mat & w, int xtype, const void * x, int64_t ldx, int64_t x_rows, const moe_view * v,

@@ -20,8 +20,6 @@
 // half that, in a ring of four, took 9 % longer.
 #include "mx4.h"
 
-#include <algorithm>
-#include <cmath>
 #include <utility>
 
 namespace mi355x_ops {
@@ -326,59 +324,13 @@ static hipError_t run_tile(const mx4_args & a, int shares, float * part, int yty
     });
 }
 
-// Which tile: the one whose time, by what a CU was measured to take (us), comes out least.  A plane
-// (256 of K) takes 2.1 in a 256 x 256 tile, 0.65 in a 128 x 128 tile alone on its CU and 0.8 in one of
-// several, 0.33 and 0.26 in 64 x 64 tiles; beginning and end add 8, 4 and 4.  Tiles come in whole rounds
-// of the CUs; experts' are counted as half full at their ends, a quarter of a tile each, since waves
-// without rows cost little, and the routing's rounds as half one more.  Large tiles move the least
-// bytes for their products, small ones give more CUs work: 512 x 28672 x 4096 takes 38 us in tiles of
-// 256 and 50 in tiles of 128, 1024 x 4096 x 4096 25 and 15, 256 x 4096 x 4096 24 and 14, in tiles of 64 9.5;
-// 8192 pairs by 8 experts of 4096 x 14336 335 in tiles of 256, 382 in tiles of 128.
-// Deep rings serve CUs that have one tile (512 x 4096 x 14336: 38 us with four planes, 58 with two),
-// shallow ones let several share a CU (2048 x 4096 x 4096: 27 and 24; experts' tiles of 64, 300 tokens
-// by 8 experts of 4096 x 4096: 24 and 20).
-// A long K over few tiles is cut into shares whose sums a second kernel joins: 128 x 4096 x 14336 22 -> 18
-// us, 64 x 4096 x 14336 24 -> 14, 100 x 640 x 14336 21 -> 10.5.
-struct tile_choice {
-    int side, stages, shares;
-};
-
-static tile_choice pick_tile(const mx4_args & a, bool ids) {
-    constexpr double CUS = 256;
-    const int planes = (a.KB + 7) / 8;
-    auto rounds = [&](double n) { return ids ? std::max(n + 0.5, 1.0) : std::ceil(n); };
-    tile_choice best = {};
-    double least = 0;
-    for (const int side : {256, 128, 64}) {
-        const int64_t busy = std::min(a.T, (int64_t) a.n_expert);
-        const double cols = ids ? (double) a.T / side + 0.25 * busy : (double) ((a.T + side - 1) / side);
-        const double tiles = cols * ((a.M + side - 1) / side) / CUS;   // for each CU
-        for (int shares = 1; shares <= 16 && (shares == 1 || planes >= 2 * shares); shares *= 2) {
-            const double n = tiles * shares, p = (planes + shares - 1) / shares;
-            double t;
-            if (side == 256) t = rounds(n) * (p * 2.1 + 8);
-            else if (side == 128) t = n <= 1 ? rounds(n) * (p * 0.65 + 4) : rounds(n) * p * 0.8 + rounds(n / 2) * 4;
-            else t = n <= 1 ? rounds(n) * (p * 0.33 + 4) : rounds(n) * p * 0.26 + rounds(n / 4) * 4;
-            // the join: a launch, and the sums written and read
-            if (shares > 1) t += 3 + (double) shares * a.T * a.M * 8 / 4e6;
-            if (least == 0 || t < least) {
-                least = t;
-                best = {side, side == 256 ? 2 : side == 128 ? (n <= 1 ? 4 : 2) : (ids ? 2 : 4), shares};
-            }
-        }
-    }
-    // every share has planes of its own
-    while (best.shares > 1 && (planes + best.shares - 1) / best.shares * (best.shares - 1) >= planes) best.shares /= 2;
-    return best;
-}
-
 int64_t mx4_tile_workspace(const mx4_args & a) {
-    const tile_choice c = pick_tile(a, a.n_expert != 0);
+    const tile_choice c = pick_tile(a);
     return c.shares > 1 ? c.shares * a.T * a.M * (int64_t) sizeof(float) : 0;
 }
 
 template <bool IDS> static hipError_t product_tile(const mx4_args & a, float * part, int ytype, hipStream_t st) {
-    const tile_choice c = pick_tile(a, IDS);
+    const tile_choice c = pick_tile(a);
     if (c.side == 256) return run_tile<4, 2, 2, 4, 2, IDS>(a, c.shares, part, ytype, st);
     if (c.side == 128 && c.stages == 4) return run_tile<2, 2, 2, 2, 4, IDS>(a, c.shares, part, ytype, st);
     if (c.side == 128) return run_tile<2, 2, 2, 2, 2, IDS>(a, c.shares, part, ytype, st);

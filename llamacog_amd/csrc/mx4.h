@@ -3,6 +3,7 @@
 #pragma once
 
 #include "devops.h"
+#include "mx4_rules.h"
 
 namespace mi355x_ops {
 
@@ -85,19 +86,15 @@ __device__ __forceinline__ v4f mfma_mx4_16(const int4 & a, const int4 & b, v4f c
 }
 
 // ---- arguments of the products ---------------------------------------------------------------
-struct mx4_args {
+struct mx4_args : product_size {
     const uint8_t * w_codes;
     const uint8_t * w_scales;
     int64_t w_codes_stride, w_scales_stride;   // from one expert's matrix to the next
-    int64_t M;
-    int KB;                                    // K / 32
     const uint8_t * x_codes;
     const uint8_t * x_scales;
     int64_t x_rows;                            // rows of the x matrix (its scale planes' stride)
-    int64_t T;                                 // rows of y
     const int32_t * order;
     const int32_t * offsets;
-    int n_expert;
     int used;                                  // 0: x rows are in sorted order
     void * y;
 };
@@ -105,10 +102,6 @@ struct mx4_args {
 // k_mx4_gemm.hip; by experts where a.n_expert is not 0.  part: mx4_tile_workspace(a) bytes
 int64_t mx4_tile_workspace(const mx4_args & a);
 hipError_t mx4_product_tile(const mx4_args & a, float * part, int ytype, hipStream_t st);
-
-// bytes of an x row in shared memory: codes and exponents, an odd number of 16-B columns, so that the
-// same column of 16 rows lies in 16 different ones of the banks
-__host__ __device__ constexpr int mv_row_bytes(int KB) { return (KB + (KB + 15) / 16 | 1) * 16; }
 
 // ---- tiles of sorted pairs -------------------------------------------------------------------
 struct tile_rows {
