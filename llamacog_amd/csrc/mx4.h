@@ -130,7 +130,7 @@ struct tile_scan {
         e0 = min(lane * per, a.n_expert);
         e1 = min(e0 + per, a.n_expert);
         mine = 0;
-        for (int e = e0; e < e1; ++e) mine += (a.offsets[e + 1] - a.offsets[e] + rows - 1) / rows;
+        for (int e = e0; e < e1; ++e) mine += tiles_of(a.offsets[e + 1] - a.offsets[e], rows);
         upto = mine;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -158,7 +158,7 @@ struct tile_scan {
             int left = (int) i - (upto - mine);
             for (;; ++e) {
                 n = a.offsets[e + 1] - a.offsets[e];
-                const int t = (n + rows - 1) / rows;
+                const int t = tiles_of(n, rows);
                 if (left < t || e + 1 >= e1) break;
                 left -= t;
             }

@@ -15,6 +15,9 @@ struct product_size {
     int n_expert;   // 0: dense
 };
 
+// tiles of `rows` rows that hold n, which may be close to 2^31
+constexpr int tiles_of(int n, int rows) { return n / rows + (n % rows > 0); }
+
 // ---- few rows (k_mx4.hip) --------------------------------------------------------------------
 constexpr int MV_WAVES = 8;              // of a workgroup
 constexpr int64_t MV_LDS = 144 * 1024;   // most shared memory of a workgroup, of a CU's 160 KiB

@@ -97,6 +97,13 @@ def test_each_kernel_has_its_sizes(tmp_path):
     assert {v for s, v in FEW.items() if s[3]} == {(1, k) for k in (1, 2, 4, 8)}
 
 
+def test_tiles_of_nearly_all_32_bits(tmp_path):
+    """One expert's pairs may be as many as 2^31 - 1: their tiles are counted without passing 32 bits."""
+    cases = [(0, 64), (1, 64), (64, 64), (65, 64), (2 ** 31 - 1, 256), (2 ** 31 - 16, 64), (2 ** 31 - 64, 64), (2 ** 31 - 1, 16)]
+    checks = "".join(f"static_assert(mi355x_ops::tiles_of({n}, {rows}) == {-(-n // rows)});" for n, rows in cases)
+    compiled(tmp_path, f'#include "mx4_rules.h"\n{checks} int main() {{}}')
+
+
 # ---- on the GPU ----------------------------------------------------------------------------------
 def octaves(k):
     """How far exponents may lie from 1 with whole sums of K products: on average a product is 5.06 times
