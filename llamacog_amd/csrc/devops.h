@@ -66,11 +66,11 @@ hipError_t moe_combine_back(int type, const void * dy, int64_t lddy, const void 
                             int used, const int32_t * order, const int32_t * rank, const float * w, void * dys, float * dw,
                             hipStream_t st);
 
-// A launch counts its threads in 32 bits along each axis.  Row groups of 256 threads, which may be more
-// than that, lie along x and z: group row_group() of row_groups(n, y).
+// A launch counts its threads in 32 bits along each axis.  Groups of `waves` waves, which may be more
+// than that, lie along x and z: group group_id() of row_groups(n, y, waves), some of them past n.
 constexpr int64_t MAX_WAVES = ((int64_t) 1 << 32) / 64 - 1;
-static inline dim3 row_groups(int64_t n, int64_t y) {
-    const int64_t z = (n + MAX_WAVES / 4 - 1) / (MAX_WAVES / 4);
+static inline dim3 row_groups(int64_t n, int64_t y, int waves = 4) {
+    const int64_t z = (n + MAX_WAVES / waves - 1) / (MAX_WAVES / waves);
     return dim3((unsigned) ((n + z - 1) / z), (unsigned) y, (unsigned) z);
 }
 
@@ -90,7 +90,7 @@ static inline hipError_t launch(void (*kernel)(P...), dim3 grid, unsigned thread
 }
 
 // ---- device side -----------------------------------------------------------------------------
-__device__ __forceinline__ int64_t row_group() { return (int64_t) blockIdx.z * gridDim.x + blockIdx.x; }
+__device__ __forceinline__ int64_t group_id() { return (int64_t) blockIdx.z * gridDim.x + blockIdx.x; }
 
 template <class T> __device__ __forceinline__ float to_f32(T v) { return (float) v; }
 template <class T> __device__ __forceinline__ T from_f32(float v) { return (T) v; }   // to nearest, ties to even

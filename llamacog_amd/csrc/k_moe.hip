@@ -208,7 +208,7 @@ template <class T> constexpr int COLS = 16 / sizeof(T);
 
 static __device__ __forceinline__ bool my_columns(const row_args & a, int N, int64_t & t, int64_t & col) {
     col = ((int64_t) blockIdx.y << a.lsh | (threadIdx.x & ((1 << a.lsh) - 1))) * N;
-    t = row_group() * (256 >> a.lsh) + (threadIdx.x >> a.lsh);
+    t = group_id() * (256 >> a.lsh) + (threadIdx.x >> a.lsh);
     return t < a.T && col < a.D;
 }
 
@@ -286,7 +286,7 @@ static __global__ void __launch_bounds__(256) k_moe_combine_back(row_args a, con
     constexpr int N = COLS<T>;
     __shared__ float part[4][MOE_MAX_USED];
     const int lanes = 1 << a.lsh, mine = threadIdx.x & (lanes - 1);
-    const int64_t t = row_group() * (256 >> a.lsh) + (threadIdx.x >> a.lsh);
+    const int64_t t = group_id() * (256 >> a.lsh) + (threadIdx.x >> a.lsh);
     const bool here = t < a.T;
     for (int j = blockIdx.y; j < a.used; j += gridDim.y) {
         float dot = 0.0f;

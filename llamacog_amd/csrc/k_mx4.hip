@@ -27,7 +27,7 @@ static __global__ void __launch_bounds__(256) k_mx4_quantize(const T * __restric
     const int64_t c = (int64_t) blockIdx.y << lsh | (threadIdx.x & ((1 << lsh) - 1));
     if (c >= K / 8) return;   // K / 8 is a multiple of four: the four lanes of a block stay together
     const int rp = 256 >> lsh;
-    const int64_t row0 = row_group() * rp * QROWS + (threadIdx.x >> lsh);
+    const int64_t row0 = group_id() * rp * QROWS + (threadIdx.x >> lsh);
     float v[QROWS][8];
 #pragma unroll
     for (int i = 0; i < QROWS; ++i) {
@@ -74,7 +74,7 @@ static __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t * _
     const int64_t c = (int64_t) blockIdx.y << lsh | (threadIdx.x & ((1 << lsh) - 1));
     if (c >= K / 8) return;
     const int rp = 256 >> lsh;
-    const int64_t row0 = row_group() * rp * QROWS + (threadIdx.x >> lsh);
+    const int64_t row0 = group_id() * rp * QROWS + (threadIdx.x >> lsh);
     uint32_t q[QROWS];
     unsigned e[QROWS];
 #pragma unroll

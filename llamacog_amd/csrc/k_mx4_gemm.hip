@@ -98,16 +98,18 @@ static __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tile(mx4_args a, un
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const unsigned id = (unsigned) group_id();
     unsigned tm, tn;
     tile_rows tr;
     if constexpr (IDS) {
         const tile_scan scan(a, S::TN);
         tiles_n = (unsigned) scan.tiles(a);   // the launch is for any routing
-        if (blockIdx.x >= tiles_m * tiles_n) return;
-        tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+        if (id >= tiles_m * tiles_n) return;
+        tile_of(id, tiles_m, tiles_n, tm, tn);
         tr = scan.tile(a, tn);
     } else {
-        tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+        if (id >= tiles_m * tiles_n) return;
+        tile_of(id, tiles_m, tiles_n, tm, tn);
         tr = {0, (int64_t) tn * S::TN, min((int64_t) S::TN, a.T - (int64_t) tn * S::TN)};
     }
     const int64_t m0 = (int64_t) tm * S::TM;
@@ -307,8 +309,8 @@ template <int FM, int FN, int WM, int WN, int STAGES, bool IDS>
 static hipError_t run_tile(const mx4_args & a, int shares, float * part, int ytype, hipStream_t st) {
     using S = tile_shape<FM, FN, WM, WN, STAGES>;
     const int64_t tm = (a.M + S::TM - 1) / S::TM, tn = IDS ? id_tiles(a, S::TN) : (a.T + S::TN - 1) / S::TN;
-    if (tm * tn > MAX_WAVES / S::NW) return hipErrorInvalidConfiguration;
-    const dim3 grid((unsigned) (tm * tn), shares);
+    if (tm * tn >> 32) return hipErrorInvalidConfiguration;   // no card holds these results
+    const dim3 grid = row_groups(tm * tn, shares, S::NW);
     auto go = [&](auto t, const mx4_args & a) {
         return launch(k_mx4_tile<FM, FN, WM, WN, STAGES, decltype(t), IDS>, grid, 64 * S::NW, S::LDS, st, a, (unsigned) tm, (unsigned) tn);
     };

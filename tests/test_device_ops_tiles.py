@@ -241,3 +241,42 @@ def test_tiles_in_a_graph():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(ys, want))
         assert all(torch.equal(call(), b) for call, b in zip(calls, want))
+
+
+def numbered_rows(g, rows):
+    """MXFP4 rows of 32 elements that all differ: the row's number, then a million random rows over and over."""
+    codes = torch.empty(rows, 16, dtype=torch.uint8, device="cuda")
+    some = torch.randint(0, 256, (1 << 20, 16), dtype=torch.uint8, device="cuda", generator=g)
+    for at in range(0, rows, 1 << 20):
+        codes[at:at + (1 << 20)] = some[:rows - at]
+    codes.view(torch.int32)[:, 0] = torch.arange(rows, dtype=torch.int32, device="cuda")
+    return ops.Mx4(codes, torch.full((1, rows, 8), 127, dtype=torch.uint8, device="cuda"))
+
+
+@gpu
+def test_tiles_past_32_bits_of_threads():
+    """As many rows as a call may have: more tiles than one axis of a launch has room for."""
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 110 << 30:
+        pytest.skip("110 GiB of the card's memory are wanted")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    w, _ = operand(g, (1, 32))
+    rows = 2 ** 31 - 1
+    x = numbered_rows(g, rows)
+    y = ops.mx4_mul_mat(w, x, torch.float16)
+    step = 1 << 24
+    for at in range(0, rows, step):
+        part = ops.Mx4(x.codes[at:at + step], x.scales[:, at:at + step])
+        assert torch.equal(y[at:at + step], ops.mx4_mul_mat(w, part, torch.float16)), at
+    assert y[:1 << 20].unique().numel() > 100
+    # by experts: all of 2^31 - 16 pairs but the last token's belong to one
+    tokens = rows // 16
+    y = y[:tokens].clone()
+    x = ops.Mx4(x.codes[:tokens].clone(), x.scales[:, :tokens].clone())
+    ids = torch.zeros(tokens, 16, dtype=torch.int32, device="cuda")
+    ids[-1] = -1
+    plan = ops.moe_sort(ids, 1)
+    del ids
+    ye = ops.mx4_mul_mat_id(ops.Mx4(w.codes[None], w.scales[None]), x, plan, dtype=torch.float16).view(tokens, 16)
+    assert plan.offsets.tolist() == [0, 16 * (tokens - 1)] and not ye[-1].any()
+    assert torch.equal(ye[:-1], y[:-1].expand(-1, 16))
