@@ -35,6 +35,10 @@ static int64_t sort_chunk(int64_t pairs) {   // pairs per chunk
     return c;
 }
 
+// what lanes of this wave wrote to shared memory is read by its other lanes behind this: its accesses are
+// done in order anyway, this keeps the compiler to it
+static __device__ __forceinline__ void in_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
 // the lanes of the wave whose id is this lane's
 static __device__ __forceinline__ unsigned long long same_lanes(int id, int bits) {
     unsigned long long m = ~0ull;
@@ -58,6 +62,7 @@ static __device__ __forceinline__ void for_run(const I * ids, int64_t p0, int64_
             if (p + 64 * i >= p1) break;
             const int id = v[i] >= 0 && v[i] < (I) n_expert ? (int) v[i] : -1;
             f(p + 64 * i + lane, id, same_lanes(id, bits));
+            in_order();   // the next 64 count on from what these wrote
         }
     }
 }
@@ -97,6 +102,7 @@ static __global__ void __launch_bounds__(64 * SORT_WAVES) k_moe_sort(const I * _
     const int64_t p0 = min(c0 + wave * run, c1), p1 = min(p0 + run, c1);
     int * mine = cnt + wave * n_expert;
     for (int i = lane; i < n_expert; i += 64) mine[i] = 0;
+    in_order();
     for_run(ids, p0, p1, n_expert, bits, [&](int64_t, int id, unsigned long long m) {
         if (id >= 0 && __builtin_ctzll(m) == lane) mine[id] += __popcll(m);
     });
