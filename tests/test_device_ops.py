@@ -931,3 +931,84 @@ def test_only_the_binding_is_built_against_torch(target, binding):
     out = subprocess.run(["make", "-n", "-B", "-C", csrc, target], capture_output=True, text=True, check=True).stdout
     assert ("torch" in re.sub(r"make.*directory.*", "", out)) == binding
     assert "libmi355x-ops.so" in out
+
+
+@gpu
+def test_every_exponent():
+    """All codes with all exponents as values, and as products of one block: zeros under float32's least number,
+    infinities past its largest, NaN for 255; tiles and few rows."""
+    rng = np.random.default_rng(4)
+    byte = np.arange(256, dtype=np.uint8)[:, None]
+    code = np.tile(np.arange(16, dtype=np.uint8), 2)[None].repeat(256, 0)
+    with np.errstate(over="ignore"):
+        want = torch.from_numpy(np_values(code, byte))
+    for dtype in TYPES:
+        y = ops.mx4_dequantize(pack(code, byte), dtype).cpu()
+        assert torch.equal(y.nan_to_num(99.0), want.to(dtype).nan_to_num(99.0)) and torch.equal(y.isnan(), want.isnan())
+    cw, cx = rng.integers(0, 16, (2, 256, 32), dtype=np.uint8)
+    s = GRID[cx] @ GRID[cw].T                 # exact, and so is its product with a power of two in 64 bits
+    with np.errstate(over="ignore"):
+        want = np.ldexp(s, byte.astype(int) + byte.T.astype(int) - 254).astype(np.float32)
+    want[255] = want[:, 255] = np.nan
+    for t in (1, 16, 32, 256):
+        for at in range(0, 256, max(t, 32)):
+            rows = slice(at, at + t)
+            y = ops.mx4_mul_mat(pack(cw, byte), pack(cx[rows], byte[rows]), torch.float32).cpu().numpy()
+            assert np.array_equal(y, want[rows], equal_nan=True)
+
+
+@gpu
+def test_tensors_without_rows_or_columns():
+    rng = np.random.default_rng(0)
+    w, _ = random_mx4(rng, 8, 64)
+    we, _ = random_mx4(rng, 3, 8, 64)
+    none_w = ops.Mx4(w.codes[:0], w.scales[:, :0].contiguous())
+    none_e = ops.Mx4(we.codes[:, :0].contiguous(), we.scales[:, :, :0].contiguous())
+    x, weights = torch.ones(4, 64, device="cuda"), torch.ones(4, 2, device="cuda")
+    _, _, _, plan = plan_of(rng, 4, 2, 3, "even")
+    no_plan = ops.moe_sort(torch.zeros(0, 2, dtype=torch.int32, device="cuda"), 3)
+    q = ops.mx4_quantize(x[:0])
+    assert q.codes.shape == (0, 32) and q.scales.shape == (1, 0, 8) and ops.mx4_dequantize(q).shape == (0, 64)
+    assert ops.mx4_mul_mat(w, x[:0]).shape == ops.mx4_mul_mat(w, q).shape == (0, 8) and ops.mx4_mul_mat(none_w, x).shape == (4, 0)
+    assert ops.mx4_mul_mat_id(we, x[:0], no_plan).shape == (0, 8) and ops.mx4_mul_mat_id(none_e, x, plan).shape == (8, 0)
+    assert ops.moe_gather(x[:, :0], plan).shape == (8, 0) and ops.moe_combine(x.repeat(2, 1)[:, :0], plan, weights).shape == (4, 0)
+    dys, dw = ops.moe_combine_back(x[:0], x[:0], no_plan, weights[:0])
+    assert dys.shape == (0, 64) and dw.shape == (0, 2)
+    dys, dw = ops.moe_combine_back(x[:, :0], x.repeat(2, 1)[:, :0], plan, weights)
+    assert dys.shape == (8, 0) and not dw.any()          # a sum of nothing
+
+
+@gpu
+def test_large_expert_layer_in_a_graph():
+    """Two launches of the sort, products in tiles; replayed on new routings with eager work between."""
+    args, _ = layer_case(3000)
+    x, ids, weights = (v.clone() for v in args[:3])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        expert_layer(x, ids, weights, *args[3:])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = expert_layer(x, ids, weights, *args[3:])
+    for seed in range(3):
+        fresh, _ = layer_case(3000, seed)
+        for to, src in zip((x, ids, weights), fresh[:3]):
+            to.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, expert_layer(x, ids, weights, *args[3:]))
+
+
+@gpu
+def test_weights_of_experts_stacked():
+    """The experts' weights out of one quantisation each, as the documentation stacks them."""
+    rng = np.random.default_rng(6)
+    matrices = [rows_of(rng, 40, 288, torch.bfloat16)[0] for _ in range(3)]
+    w = ops.Mx4(*map(torch.stack, zip(*map(ops.mx4_quantize, matrices))))
+    ids, order, _, plan = plan_of(rng, 20, 2, 3, "even")
+    x, x64 = rows_of(rng, 20, 288, torch.float32)
+    y = ops.mx4_mul_mat_id(w, x, plan)
+    for e in range(3):
+        at = np.flatnonzero(ids.reshape(-1)[order] == e)
+        check_product(y[torch.from_numpy(at).cuda()], np_rounded(matrices[e].double().cpu().numpy()), np_rounded(x64)[order[at] // 2], torch.float32)
