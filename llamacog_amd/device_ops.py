@@ -16,12 +16,36 @@ gradient is recorded: an input that asks for one, or carries a tangent of forwar
 from __future__ import annotations
 
 import ctypes
+import glob
+import importlib.util
 import os
+import sys
 from typing import NamedTuple
 
-import torch
 
-from . import PKG, BackendMissing
+def _hip_runtimes() -> set[str]:
+    with open("/proc/self/maps") as maps:
+        return {os.path.realpath(line.split()[-1]) for line in maps if "libamdhip64" in line}
+
+
+def _refuse(runtimes: set[str]):
+    raise ImportError("two HIP runtimes in this process: import llamacog_amd.device_ops (or torch) before the plugin is loaded: "
+                      + ", ".join(sorted(runtimes)))
+
+
+# torch brings a HIP runtime of its own.  The plugin, loaded later, uses that one too; loaded before, it
+# has brought the system's, and two runtimes in a process do not know of each other's work (and may abort it
+# at its end): torch is not imported then.
+if "torch" not in sys.modules and _hip_runtimes():
+    _torch = importlib.util.find_spec("torch")
+    _own = {os.path.realpath(f) for d in (_torch.submodule_search_locations if _torch else ())
+            for f in glob.glob(os.path.join(d, "lib", "libamdhip64.so*"))}
+    if _own and not _own & _hip_runtimes():
+        _refuse(_own | _hip_runtimes())
+
+import torch  # noqa: E402
+
+from . import PKG, BackendMissing  # noqa: E402
 
 LIBRARY = os.path.join(PKG, "libmi355x-ops.so")   # the flat ABI
 BINDING = os.path.join(PKG, "_device_ops.so")     # csrc/devops_torch.cpp
@@ -38,13 +62,8 @@ if not os.path.exists(BINDING):
     raise BackendMissing(f"operators not built: {BINDING} is missing (run __graft_entry__.build())")
 from . import _device_ops as _ops  # noqa: E402
 
-# torch brings a HIP runtime of its own.  The plugin, loaded later, uses that one too; loaded before, it
-# has brought the system's, and two runtimes in a process do not know of each other's work.
-with open("/proc/self/maps") as _maps:
-    _runtimes = {line.split()[-1] for line in _maps if "libamdhip64" in line}
-if len(_runtimes) > 1:
-    raise ImportError("two HIP runtimes in this process: import llamacog_amd.device_ops (or torch) before the plugin is loaded: "
-                      + ", ".join(sorted(_runtimes)))
+if len(_hip_runtimes()) > 1:
+    _refuse(_hip_runtimes())
 
 
 class Mx4(NamedTuple):

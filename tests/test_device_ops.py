@@ -10,6 +10,7 @@ import ctypes
 import os
 import re
 import subprocess
+import sys
 import threading
 
 import numpy as np
@@ -1012,3 +1013,21 @@ def test_weights_of_experts_stacked():
     for e in range(3):
         at = np.flatnonzero(ids.reshape(-1)[order] == e)
         check_product(y[torch.from_numpy(at).cuda()], np_rounded(matrices[e].double().cpu().numpy()), np_rounded(x64)[order[at] // 2], torch.float32)
+
+
+def test_a_second_hip_runtime_is_refused_before_it_is_loaded():
+    """The flat library (as the plugin would) has brought the system's runtime: torch's is not loaded beside it."""
+    code = f"""
+import ctypes, sys
+ctypes.CDLL({ops.LIBRARY!r}, mode=ctypes.RTLD_GLOBAL)
+sys.path.insert(0, {la.REPO!r})
+try:
+    import llamacog_amd.device_ops
+    print("imported")
+except ImportError as e:
+    print("refused" if "two HIP runtimes" in str(e) else e, "torch" in sys.modules)
+"""
+    if not os.path.exists(os.path.join(os.path.dirname(torch.__file__), "lib", "libamdhip64.so")):
+        pytest.skip("this torch brings no HIP runtime of its own")
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert out.returncode == 0 and out.stdout.split() == ["refused", "False"], (out.returncode, out.stdout, out.stderr)
