@@ -22,8 +22,9 @@ static inline unsigned ceil_div(int64_t a, int64_t b) { return (unsigned) ((a + 
 // One chunk is one launch; more are two: the chunks' counts, then their places, where every
 // workgroup sums the counts in front of its own (at most SORT_CHUNKS of them).  Bound by latency:
 // ids are loaded SORT_LOADS at a time, the chunks' counts are summed by all threads.  2 pairs 3.2 us,
-// 4000 5.8, 131072 by 128 experts 15 (both launches).  Chunks of 8192 and 16384 took longer: 4000 pairs
-// 8.3 and 13.3 us a call instead of 6.4, 16000 11.5 and 16.8 instead of 11.5.
+// 131072 by 128 experts 15.5 (4.8 and 10.7).  Whole calls with chunks of 1024 / 2048 / 4096 pairs: 4000 by 8 experts
+// 8.1 / 9.0 / 6.4 us, 4000 by 128 7.5 / 9.3 / 8.4, 16384 by 64 8.0 / 9.2 / 12.5, 131072 by 128 9.9 / 10.8 / 14.8,
+// 524288 by 256 19.7 / 18.6 / 18.9; with chunks of 8192 4000 took 8.3.
 constexpr int SORT_WAVES = 16;
 constexpr int SORT_LOADS = 4;
 constexpr int SORT_CHUNK = SORT_WAVES * SORT_LOADS * 64;    // least pairs of a chunk
@@ -202,9 +203,10 @@ hipError_t moe_sort(const void * ids, int id_bytes, int64_t pairs, int n_expert,
 // All three are bound by memory: every row is read once and written once, a token's row once for
 // all of its slots (the gather goes by rank, not by order, for that).  A lane owns 16 bytes of a
 // token's columns, the last one what is left; lanes are laid over the columns in a power of two.
-// Rows lie on any address.  16384 tokens, 8 slots, 2048 bf16 columns: gather 102 us (5.9 TB/s, nearly all
-// writes, past the caches: 112 through them), combine 127 (4.7 TB/s), back 228 (5.0 TB/s); with 2047
-// columns 142, 137 and 307.
+// Rows lie on any address.  16384 tokens, 8 slots, 2048 bf16 columns: gather 103 us (5.9 TB/s, nearly all
+// writes, past the caches: 112 through them), combine 127 - 132 (4.7 TB/s), back 230 (5.0 TB/s).  With 2047 columns
+// 148, 143 and 316, with 2046 142, 137 and 288: rows begin anywhere in a cache line, and most 16-byte accesses are
+// not aligned to their size.
 struct row_args {
     int64_t T, D, pairs;
     int used, lsh;   // slots; log2 of the lanes over a row
@@ -371,6 +373,8 @@ hipError_t moe_combine_back(int type, const void * dy, int64_t lddy, const void 
         // here a lane may have several columns: no more lanes than columns, so that none is idle for long
         if (a.lsh > 0 && ((int64_t) COLS<E> << a.lsh) > D + COLS<E> - 1) --a.lsh;
         const int64_t n = ceil_div(T, 256 >> a.lsh);
+        // slots side by side or one after the other: 512 tokens of 8 x 2048 bf16 9.8 us and 16.0, 1024 15.7 and 18.7,
+        // 2000 28.3 both, 4096 62.0 and 59.6
         const dim3 groups = row_groups(n, n < 2048 ? used : 1);
         return launch(k_moe_combine_back<E, whole, flag>, groups, 256, 0, st, a, (const E *) dy, lddy, (const E *) ys, ldys, order, rank, w,
                       (E *) dys, dw);

@@ -17,8 +17,9 @@ static inline unsigned ceil_div(int64_t a, int64_t b) { return (unsigned) ((a + 
 // 16-B load of the 16-bit types), four lanes a block: their maximum is two DPP steps, and the
 // conversion is the hardware's (v_cvt_scalef32_pk_fp4: one rounding, saturating).  Lanes are laid
 // over a row's columns in a power of two so that no division is needed; a workgroup takes QROWS
-// times as many rows as its lanes hold, loads first, to keep bytes in flight.  28672 x 8192: 118 us from
-// bf16, 5.0 TB/s, the rate of a copy; 230 us from float32, 4.6 TB/s.
+// times as many rows as its lanes hold, loads first, to keep bytes in flight.  28672 x 8192: 120 us from
+// bf16, 5.0 TB/s, the rate of a copy; 234 us from float32, 4.5 TB/s.  Right behind a kernel that has written 470 MB
+// the first takes 143 (median; 122 at least).
 constexpr int QROWS = 4;
 
 template <class T>
@@ -67,7 +68,7 @@ hipError_t mx4_quantize(int type, const void * x, int64_t ldx, int64_t rows, int
 }
 
 // ---- values back -----------------------------------------------------------------------------
-// Bound by memory, laid out as the quantisation is: 28672 x 8192 to bf16 117 us, 5.0 TB/s.
+// Bound by memory, laid out as the quantisation is: 28672 x 8192 to bf16 119 us, 5.0 TB/s.
 template <class T>
 static __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t * __restrict__ codes, const uint8_t * __restrict__ scales,
                                                         int64_t rows, int64_t K, int lsh, T * __restrict__ y) {
@@ -116,8 +117,9 @@ hipError_t mx4_dequantize(const mx4_mat & m, int type, void * y, hipStream_t st)
 // The x rows come as MXFP4, or as floats that every workgroup quantises for itself behind its first
 // weight loads: that costs a little arithmetic in each and saves a launch.
 //
-// One row: 4096 x 14336 9.5 us, 28672 x 4096 14.5 (4.3 TB/s), two experts of 28672 x 4096 25 (5.0 TB/s): about
-// 3 us until the first weights have come, then the memory's rate.
+// One row, weights that no cache holds: 4096 x 14336 10.7 us, 28672 x 4096 14.4 (4.3 TB/s), two experts of 28672 x
+// 4096 26 (4.8 TB/s): about 3 us until the first weights have come, then the memory's rate.  The same weights call
+// after call, which the 256-MB cache then holds in part: 9.7, 13.7 and 25.
 
 // U planes of a row group
 template <int U> struct mv_weights {
@@ -252,7 +254,7 @@ static hipError_t run_mv(const mx4_args & a, const X * x, int64_t ldx, int ytype
         auto go = [&](auto split) {
             constexpr int KS = split;
             const int64_t rounds = ((a.M + 15) / 16 + MV_WAVES / KS - 1) / (MV_WAVES / KS);
-            const int64_t fair = (768 + busy - 1) / busy;   // three workgroups per CU in all, each with its turn of the groups
+            const int64_t fair = (MV_GROUPS + busy - 1) / busy;   // each with its turn of the groups
             const int per_tile = (int) (rounds < fair ? rounds : fair);
             if (per_tile * tiles > MAX_WAVES / MV_WAVES) return hipErrorInvalidConfiguration;
             return launch(k_mx4_mv<NT, KS, X, Y, IDS>, (unsigned) (per_tile * tiles), 64 * MV_WAVES, mv_lds(a, NT, KS), st, a, x, ldx,

@@ -14,10 +14,11 @@
 //     that belongs in its slot.
 //   - Past K both exponents are 0, so that the product of two codes vanishes (2^-254 of it).
 //   - Past M and T rows repeat the last one; their results are not stored.
-// Bound by power: on random codes the card holds this kernel at 1.6 - 1.7 GHz (2.2 on zeros, where it takes
-// 0.71 of the time), as it does the instruction alone (6.15 PFLOP/s).  2048 x 28672 x 8192 255 us, 3.8
-// PFLOP/s; 4096 x 4096 x 28672 247 us, 3.9 PFLOP/s.  A row's 128 B of a plane are a whole cache line: planes of
-// half that, in a ring of four, took 9 % longer.
+// Bound by cycles: 2048 x 28672 x 8192 takes 432 thousand of them on random codes and 436 on zeros (251 and 193 us:
+// the clock is 1.72 and 2.27 GHz), and the matrix cores are busy for 229 thousand, 53 %.  An eighth is the last round of
+// tiles, half full; of a plane's about 3000 cycles in a 256 x 256 tile the matrix cores have 2048.  251 us are 3.8
+// PFLOP/s, 4096 x 4096 x 28672 in 217 us 4.4; the instruction alone reaches 6.15 on random codes.  A row's 128 B of
+// a plane are a whole cache line: planes of half that, in a ring of four, took 9 % longer.
 #include "mx4.h"
 
 #include <utility>
@@ -81,7 +82,9 @@ static __device__ __forceinline__ void mma_step(v16f (&acc)[FM][FN], const frags
 
 // Workgroup -> tile.  Consecutive workgroups go round the eight XCDs: each XCD gets one run of the
 // tiles, so that what its workgroups share meets in its L2.  A run goes along GROUP x tiles, then
-// to the next weight tile: the 32 that an XCD has at a time are about 4 by 8.
+// to the next weight tile: the 32 that an XCD has at a time are about 4 by 8.  With GROUP 1 / 4 / 8 / 16,
+// 2048 x 28672 x 8192 took 275 / 274 / 272 / 271 us, 4096 x 4096 x 28672 218 / 217 / 217 / 227, 2048 x 14336 x 4096
+// 76 / 74 / 73 / 77.
 static __device__ __forceinline__ void tile_of(unsigned id, unsigned tiles_m, unsigned tiles_n, unsigned & tm, unsigned & tn) {
     constexpr unsigned GROUP = 8;
     const unsigned n = tiles_m * tiles_n, xcd = id & 7;

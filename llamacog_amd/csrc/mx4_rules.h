@@ -36,9 +36,14 @@ inline int64_t mv_busy(const product_size & a, int NT) {
     return a.n_expert ? std::min(a.T, (int64_t) a.n_expert) : (a.T + 16 * NT - 1) / (16 * NT);
 }
 
+// Workgroups in all: three for a CU.  With 256 / 512 / 768 / 1024 / 1536, 28672 x 4096 by one row takes 16.1 / 14.5 /
+// 14.5 / 14.5 / 14.5 us, 32001 x 4096 by 29 rows 23.1 / 21.4 / 21.3 / 21.6 / 21.4, 800 pairs by 128 experts of
+// 1408 x 2048 66 / 54 / 51 / 58 / 46.
+constexpr int64_t MV_GROUPS = 768;
+
 // how many waves share a group of 16 weight rows: as few as give the tiles MV_FILL waves in all.  With
-// 1024 / 2048 / 4096 / 8192, 4096 x 14336 by one row took 13.3 / 10.7 / 10.7 / 10.7 us, 32001 x 4096 by 29 rows
-// 21.1 / 21.1 / 22.2 / 21.5, 4096 x 14336 by 64 39 / 26 / 31 / 34.
+// 1024 / 2048 / 4096 / 8192, 4096 x 14336 by one row takes 13.5 / 10.9 / 10.8 / 10.8 us, by 16 rows (quantised
+// before) 18.9 / 16.3 / 16.2 / 16.3, 32001 x 4096 by 29 rows 21.5 / 21.3 / 26.9 / 27.7.
 constexpr int64_t MV_FILL = 2048;
 inline int mv_split(const product_size & a, int NT) {
     const int64_t groups = (a.M + 15) / 16 * mv_busy(a, NT);
@@ -47,17 +52,24 @@ inline int mv_split(const product_size & a, int NT) {
     return ks;
 }
 
-// The kernel for few rows, as long as its tiles of 16 or 32 rows read the weights about once: 4096 x
-// 4096 by 20 rows takes 5.6 us here and 9.2 in 64 x 64 tiles, 28672 x 4096 by 64 rows 28.6 and 18.5;
-// by experts up to 16 rows each.
+// The kernel for few rows: up to 32, by experts up to 16 each on average.  4096 x 4096 by 20 and 32 rows takes 6.1
+// and 6.5 us here, 8.0 and 9.1 in the tiles below; 28672 x 4096 by 33 and 64 rows 25 and 26, there 16 and 17; 256 pairs
+// by 256 experts of 1408 x 2048, evenly, 49 and 54.  It is not always the faster one: 28672 x 4096 by 32 rows 18.0
+// and 15.8, 4096 x 14336 by 17 and 32 rows (the 32 in two tiles, each of which reads the weights) 15.3 and 15.8,
+// there 12.7 and 12.2.  Nor does it look at the routing, which is on the device: those 256 pairs all on one expert take 25
+// and 12, 2048 pairs by 128 experts 60 and 44 evenly, 56 and 41 with nine in ten on eight of them.
 inline bool few_rows(const product_size & a) {
     return a.T <= (a.n_expert ? 16 * (int64_t) a.n_expert : 32) && mv_lds(a, 1, MV_WAVES) <= MV_LDS;
 }
 
-// few enough that every workgroup may quantise those of its tile
+// Few enough that every workgroup may quantise those of its tile, which saves a launch.  4096 x 14336 by 1 / 2 / 3 /
+// 4 / 8 float32 rows 10.9 / 12.2 / 13.6 / 14.8 / 20.7 us so, 13.3 / 13.6 / 13.8 / 13.9 / 14.1 with a launch for them;
+// 28672 x 4096 by bf16 rows 14.6 / 15.9 / 16.0 / 16.2 / 18.2 and 17.4 / 17.3 / 17.3 / 17.4 / 17.7.  By experts a
+// workgroup has only its own expert's: 16 pairs by 8 experts of 28672 x 4096 87 and 89, 12 by 64 of 1408 x 2048 9.2
+// and 11.2, 48 of the latter 15.7 and 18.0.
 inline bool float_rows(const product_size & a) { return few_rows(a) && a.T <= (a.n_expert ? 16 : 2); }
 
-// how many tiles of 16 x rows a workgroup keeps: two where they fit, so that the weights are read once
+// how many tiles of 16 x rows a workgroup keeps: two where they fit (32 up to K = 8160), so that the weights are read once
 inline int mv_tiles(const product_size & a) { return !a.n_expert && a.T > 16 && mv_lds(a, 2, MV_WAVES) <= MV_LDS ? 2 : 1; }
 
 // ---- tiles (k_mx4_gemm.hip) ------------------------------------------------------------------
@@ -66,14 +78,14 @@ inline int mv_tiles(const product_size & a) { return !a.n_expert && a.T > 16 && 
 // several, 0.33 and 0.26 in 64 x 64 tiles; beginning and end add 8, 4 and 4.  Tiles come in whole rounds
 // of the CUs; experts' are counted as half full at their ends, a quarter of a tile each, since waves
 // without rows cost little, and the routing's rounds as half one more.  Large tiles move the least
-// bytes for their products, small ones give more CUs work: 512 x 28672 x 4096 takes 38 us in tiles of
-// 256 and 50 in tiles of 128, 1024 x 4096 x 4096 25 and 15, 256 x 4096 x 4096 24 and 14, in tiles of 64 9.5;
-// 8192 pairs by 8 experts of 4096 x 14336 335 in tiles of 256, 382 in tiles of 128.
-// Deep rings serve CUs that have one tile (512 x 4096 x 14336: 38 us with four planes, 58 with two),
-// shallow ones let several share a CU (2048 x 4096 x 4096: 27 and 24; experts' tiles of 64, 300 tokens
-// by 8 experts of 4096 x 4096: 24 and 20).
-// A long K over few tiles is cut into shares whose sums a second kernel joins: 128 x 4096 x 14336 22 -> 18
-// us, 64 x 4096 x 14336 24 -> 14, 100 x 640 x 14336 21 -> 10.5.
+// bytes for their products, small ones give more CUs work: 512 x 28672 x 4096 takes 41 us in tiles of
+// 256, 54 in tiles of 128 and 83 in tiles of 64, 1024 x 4096 x 4096 27, 15 and 25, 256 x 4096 x 4096 26, 12.5 and 10;
+// 8192 pairs by 8 experts of 4096 x 14336 297, 333 and 509.
+// Deep rings serve CUs that have one tile (1024 x 4096 x 4096 in tiles of 128: 15.0 us with four planes, 16.6
+// with two), shallow ones let several share a CU (2048 x 4096 x 4096: 27.5 and 24.7; in tiles of 64, 600 pairs
+// by 8 experts of 4096 x 4096 31 and 28, but 200 by 4 experts 12 and 17.5; dense 256 x 4096 x 14336 24 and 46).
+// A long K over few tiles is cut into shares whose sums a second kernel joins: 128 x 4096 x 14336 23 us whole and
+// 18 so, 64 x 4096 x 14336 23 and 13, 100 x 640 x 14336 22 and 10.
 struct tile_choice {
     int side, stages, shares;
 };

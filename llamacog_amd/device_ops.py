@@ -101,7 +101,8 @@ def mx4_quantize(x: torch.Tensor) -> Mx4:
 
 
 def mx4_dequantize(m: Mx4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
-    """The values [rows, K] that MXFP4 rows stand for, rounded to `dtype` (exact in float32)."""
+    """The values [rows, K] that MXFP4 rows stand for, rounded to `dtype` (exact in float32, but for those past its
+    largest number, which are infinite: 2 and more under the exponent byte 254, 4 and more under 253)."""
     return _ops.dequantize(*_is(m, Mx4, "m"), dtype)
 
 
