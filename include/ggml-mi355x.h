@@ -132,8 +132,8 @@ double mi355x_bench_gemv(int wtype, int64_t K, int64_t M, int nmat, int copies, 
 double mi355x_bench_op(int which, int64_t a, int64_t b, int iters);
 
 // ---- operators on device tensors (llamacog_amd/csrc/devops_capi.cpp) -------------------------
-// MXFP4 products and expert routing.  They build no ggml node and need no ggml library: the plugin
-// exports them, and so does libmi355x-ops.so, which is these alone.  Pointers belong to the current
+// MXFP4 products and expert routing.  They build no ggml node and need no ggml library: they are
+// linked into the plugin and, alone, into libmi355x-ops.so.  Pointers belong to the current
 // device.  stream: NULL as above, MI355X_STREAM_DEFAULT the device's default stream, otherwise a
 // stream, on which the work is queued and not waited for (a captured one too).  Returns 0 or a
 // code below, and then nothing was launched unless the code is MI355X_ERR_HIP.  Element types are
