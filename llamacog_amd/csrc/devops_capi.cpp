@@ -29,9 +29,10 @@ struct call_stream {
     ~call_stream() {
         if (own) (void) hipStreamDestroy(st);
     }
+    // after a failed launch too: one in front of it may still be at work on the caller's memory
     int done(hipError_t e) {
-        if (e == hipSuccess && own) e = hipStreamSynchronize(st);
-        return e == hipSuccess ? 0 : MI355X_ERR_HIP;
+        const hipError_t waited = own ? hipStreamSynchronize(st) : hipSuccess;
+        return e == hipSuccess && waited == hipSuccess ? 0 : MI355X_ERR_HIP;
     }
 };
 

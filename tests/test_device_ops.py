@@ -1031,3 +1031,46 @@ except ImportError as e:
         pytest.skip("this torch brings no HIP runtime of its own")
     out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
     assert out.returncode == 0 and out.stdout.split() == ["refused", "False"], (out.returncode, out.stdout, out.stderr)
+
+
+# the flat ABI on launchers that do nothing: the quantisation in front of a product succeeds, the product fails
+LAUNCHERS = r"""
+#include "devops.h"
+#include "ggml-mi355x.h"
+#include <cstdio>
+static int launched, waited_for, destroyed;
+extern "C" hipError_t hipStreamCreateWithFlags(hipStream_t * s, unsigned) { *s = (hipStream_t) 16; return hipSuccess; }
+extern "C" hipError_t hipStreamSynchronize(hipStream_t) { waited_for = launched; return hipSuccess; }
+extern "C" hipError_t hipStreamDestroy(hipStream_t) { ++destroyed; return hipSuccess; }
+namespace mi355x_ops {
+hipError_t mx4_quantize(int, const void *, int64_t, int64_t, int64_t, uint8_t *, uint8_t *, hipStream_t) { ++launched; return hipSuccess; }
+mx4_needs mx4_product_needs(const mx4_mat &, int64_t, const moe_view *) { return {true, 0}; }
+hipError_t mx4_product(const mx4_mat &, const mx4_mat &, const moe_view *, int, void *, void *, hipStream_t) { return hipErrorLaunchFailure; }
+hipError_t mx4_product_float(const mx4_mat &, int, const void *, int64_t, int64_t, const moe_view *, int, void *, hipStream_t) { return hipSuccess; }
+hipError_t mx4_dequantize(const mx4_mat &, int, void *, hipStream_t) { return hipSuccess; }
+size_t moe_sort_workspace(int64_t, int) { return 0; }
+hipError_t moe_sort(const void *, int, int64_t, int, int32_t *, int32_t *, int32_t *, void *, hipStream_t) { return hipSuccess; }
+hipError_t moe_gather(int, const void *, int64_t, int64_t, int64_t, int, const int32_t *, const int32_t *, void *, hipStream_t) { return hipSuccess; }
+hipError_t moe_combine(int, const void *, int64_t, int64_t, int64_t, int, const int32_t *, const float *, void *, hipStream_t) { return hipSuccess; }
+hipError_t moe_combine_back(int, const void *, int64_t, const void *, int64_t, int64_t, int64_t, int, const int32_t *, const int32_t *, const float *,
+                            void *, float *, hipStream_t) { return hipSuccess; }
+}
+int main() {
+    uint8_t * a = (uint8_t *) (1 << 20);
+    const int rc = mi355x_mx4_mul_mat(a, a, 8, 64, 0, a, nullptr, 64, 3, 0, a, a, 1 << 20, nullptr);
+    std::printf("%d %d %d %d", rc, launched, waited_for, destroyed);
+}
+"""
+
+
+def test_private_stream_is_waited_for_after_a_failed_launch(tmp_path):
+    """What a call had launched before it failed is done when it returns: the caller may free its memory."""
+    (tmp_path / "t.cpp").write_text(LAUNCHERS)
+    csrc, objects = os.path.join(la.PKG, "csrc"), []
+    for src in (os.path.join(csrc, "devops_capi.cpp"), str(tmp_path / "t.cpp")):
+        objects.append(str(tmp_path / f"{len(objects)}.o"))
+        subprocess.run(["/opt/rocm/bin/hipcc", "-x", "hip", "--offload-host-only", "-std=c++20", "-fPIC", "-I", csrc, "-I", os.path.join(la.REPO, "include"),
+                        "-c", src, "-o", objects[-1]], check=True)
+    subprocess.run(["g++", *objects, "-o", str(tmp_path / "t")], check=True)
+    out = subprocess.run([str(tmp_path / "t")], capture_output=True, text=True, check=True).stdout
+    assert out.split() == ["-5", "1", "1", "1"]   # MI355X_ERR_HIP; one launch, waited for; the stream is gone
